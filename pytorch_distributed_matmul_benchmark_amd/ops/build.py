@@ -60,6 +60,12 @@ def _needs_build(out: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+# No packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): hipcc forms it from
+# ordinary float code, and some of its forms have given wrong results on MI355X now and then.
+# (hipcc's host pass warns that it does not know the feature; harmless.)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def experiments() -> bool:
     """``PDMB_EXPERIMENTS=1``: also compile the A/B and timing-only diagnostic
     kernels (api.h ``ExperimentKernel``). The default build ships without them."""
@@ -82,7 +88,7 @@ def source_digest() -> str:
     for p in source_files():
         h.update(p.name.encode())
         h.update(p.read_bytes())
-    h.update(f"arch={ARCH};experiments={int(experiments())}".encode())
+    h.update(f"arch={ARCH};experiments={int(experiments())};{' '.join(NO_PACKED_F32)}".encode())
     return h.hexdigest()
 
 
@@ -128,7 +134,7 @@ def build_bench(verbose: bool = False, force: bool = False) -> Path:
     obj = BUILD / "pdmb_bench.o"
     # compile and link separately: hipcc's implicit "-x hip" would otherwise
     # also apply to the kernel objects on the link line
-    _run([hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", f"-I{CSRC}",
+    _run([hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", *NO_PACKED_F32, f"-I{CSRC}",
           f"-I{rocm / 'include'}", "-c", BENCH_SRC, "-o", obj], verbose)
     _run([hipcc(), f"--offload-arch={ARCH}", obj, *objs, "-o", out, f"-L{rocm / 'lib'}", "-lrccl",
           "-lpthread", f"-Wl,-rpath,{rocm / 'lib'}"], verbose)
@@ -147,7 +153,7 @@ def build_probe(verbose: bool = False, force: bool = False) -> Path:
     32x32x16 bf16 FLOP rate on random operands (profiles/r2_mfma_shape_probe.jsonl)."""
     out = probe_path()
     if force or _needs_build(out, [PROBE_SRC]):
-        _run([hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", PROBE_SRC, "-o", out], verbose)
+        _run([hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", *NO_PACKED_F32, PROBE_SRC, "-o", out], verbose)
     return out
 
 
@@ -159,7 +165,7 @@ def build_mask_probe(verbose: bool = False, force: bool = False) -> Path:
     XCD / CU each workgroup of a CU-masked stream runs on."""
     out = RUNTIME / "cu_mask_probe"
     if force or _needs_build(out, [MASK_PROBE_SRC]):
-        _run([hipcc(), f"--offload-arch={ARCH}", "-O2", "-std=c++17", MASK_PROBE_SRC, "-o", out], verbose)
+        _run([hipcc(), f"--offload-arch={ARCH}", "-O2", "-std=c++17", *NO_PACKED_F32, MASK_PROBE_SRC, "-o", out], verbose)
     return out
 
 
@@ -173,7 +179,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
     BUILD.mkdir(exist_ok=True)
     # a flag change (PDMB_EXPERIMENTS) invalidates every object
     flags_file = BUILD / "flags.txt"
-    flags = f"arch={ARCH};experiments={int(experiments())}"
+    flags = f"arch={ARCH};experiments={int(experiments())};{' '.join(NO_PACKED_F32)}"
     if not flags_file.exists() or flags_file.read_text() != flags:
         force = True
     # Until this build links, the objects may be a mix of flavours (a failed
@@ -186,7 +192,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     hip_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
-                 "-Wno-unused-result", "-munsafe-fp-atomics", f"-I{CSRC}"]
+                 "-Wno-unused-result", "-munsafe-fp-atomics", f"-I{CSRC}", *NO_PACKED_F32]
     if experiments():
         hip_flags.append("-DPDMB_EXPERIMENTS=1")
     host_flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",

@@ -330,13 +330,16 @@ __device__ __forceinline__ void dma16_so(u32x4 rsrc, uint32_t voff, uint32_t sof
 
 // As dma16_so, but M0 is simply clobbered (declared to hipcc) instead of
 // saved and restored around every piece: 3 instructions per piece, not 5.
+// PAD: 4 wait states before the load (common.h dma16_at_pad), for pieces whose
+// soffset hipcc may have just restored from a spill with v_readlane.
+template <bool PAD = false>
 __device__ __forceinline__ void dma16_m0(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
   asm volatile(
       "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
+      "s_nop %4\n\t"
       "buffer_load_dwordx4 %0, %1, %2 offen lds"
       :
-      : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds)
+      : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds), "n"(PAD ? 3 : 0)
       : "memory", "m0");
 }
 
@@ -354,13 +357,14 @@ struct Ctx4 {
 
 // DMA piece h (0..15) of tile `tile` into stage `so`: h < 8 -> A rows
 // (h*4+wu)*8 + [0,8), else Bt rows ((h-8)*4+wu)*8 + [0,8).
+template <bool PAD = false>
 __device__ __forceinline__ void issue_piece(const Ctx4& c, int so, int tile, int h) {
   const uint32_t koff = (uint32_t)tile * BK;
   if (h < 8)
-    dma16_m0(c.ra, c.voffA, koff + (uint32_t)(h * 32 * c.lda),
+    dma16_m0<PAD>(c.ra, c.voffA, koff + (uint32_t)(h * 32 * c.lda),
              c.lds0 + so + (h * 4 + c.wu) * 8 * BK);
   else
-    dma16_m0(c.rb, c.voffB, koff + (uint32_t)((h - 8) * 32 * c.ldb),
+    dma16_m0<PAD>(c.rb, c.voffB, koff + (uint32_t)((h - 8) * 32 * c.ldb),
              c.lds0 + so + A_BYTES + ((h - 8) * 4 + c.wu) * 8 * BK);
 }
 
@@ -982,11 +986,11 @@ __global__ void __launch_bounds__(NT4, 1) gemm_fp8_sk(GemmArgs a) {
     const int nk = c.nk;
     const int t1 = nk > 1 ? 1 : 0, t2 = nk > 2 ? 2 : nk - 1;
 #pragma unroll
-    for (int h = 0; h < 16; ++h) issue_piece(c, 0, 0, h);
+    for (int h = 0; h < 16; ++h) issue_piece<true>(c, 0, 0, h);
 #pragma unroll
-    for (int h = 8; h < 16; ++h) issue_piece(c, STAGE4, t1, h);
+    for (int h = 8; h < 16; ++h) issue_piece<true>(c, STAGE4, t1, h);
 #pragma unroll
-    for (int h = 0; h < 8; ++h) issue_piece(c, STAGE4, t1, h);
+    for (int h = 0; h < 8; ++h) issue_piece<true>(c, STAGE4, t1, h);
     asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
     i32x8 A[8], A7a, A7b, B0[8], B1[8];
 #pragma unroll
@@ -997,7 +1001,7 @@ __global__ void __launch_bounds__(NT4, 1) gemm_fp8_sk(GemmArgs a) {
     A7a = A[7];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int h = 8; h < 16; ++h) issue_piece(c, 0, t2, h);
+    for (int h = 8; h < 16; ++h) issue_piece<true>(c, 0, t2, h);
     int t = 0;
     for (; t + 1 < nk; t += 2) {
       ktile_w4<0>(c, smem, t, acc, A, A7a, A7b, B0, B1, sc);
