@@ -189,6 +189,51 @@ constexpr int kMaxCopies = 16;
 hipError_t multi_copy(void* const* dsts, const void* const* srcs, const size_t* bytes, int n, int blocks_per,
                       hipStream_t stream);
 
+// Products grouped by expert (grouped.hip). Group e owns the rows [ends[e-1],
+// ends[e]) of the T rows (ends[-1] = 0; `ends` is device memory, int32 or, with
+// ends64, int64, not decreasing; values outside [0, T] are held inside it).
+//   kGroupRows:   C[r] = A[r] @ B[e]   A [T,K] at lda, B[e] [K,N] at e * sB — row stride
+//                 ldb, or b_colmajor: column stride ldb —, C [T,N] at ldc. Rows
+//                 behind the last group are left alone, or set to zero (zero_tail).
+//   kGroupReduce: C[e] = A_e^T @ B_e   A [T,M] at lda, B [T,N] at ldb, C[e] [M,N] at e * sC;
+//                 zeros for a group without rows.
+// A, B and C have the same type (kF32, kF16, kBF16); strides in elements.
+enum GroupKind : int { kGroupRows = 0, kGroupReduce = 1 };
+struct GroupedProblem {
+  int kind, dtype;
+  const void* A;
+  const void* B;
+  void* C;
+  const void* ends;
+  int ends64;
+  int E, T, M, N, K;
+  long long lda, ldb, ldc, sB, sC;
+  int b_colmajor;
+  int zero_tail;
+};
+hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream);
+
+// Products with 4-bit weights and group scales (int4.hip), 16-bit X and C:
+//   C[r] = X[r] @ W[e]^T,  W[e][n][k] = scale[e][n][k / G] * (q[e][n][k] - zero[e][n][k / G])
+// q holds two values a byte, even k in the low half: [N, K/2] bytes, 16-B aligned
+// rows of K/2; scale [N, K/G] in X's type, zero [N, K/G] bytes (nullptr: 8), both
+// contiguous, per group [E]. ends == nullptr: one group that owns all T rows;
+// otherwise as for GroupedProblem. K % G == 0, G % 32 == 0.
+struct Int4Problem {
+  int dtype;
+  const void* X;
+  const void* q;
+  const void* scale;
+  const void* zero;
+  void* C;
+  const void* ends;
+  int ends64;
+  int E, T, N, K, G;
+  long long ldx, ldc;
+  int zero_tail;
+};
+hipError_t int4_gemm(const Int4Problem& p, hipStream_t stream);
+
 // Diagnostic builds write per-wave stamps here (device memory; nullptr = off).
 void set_debug_buffer(void* p);
 

@@ -1,0 +1,120 @@
+// Matrix products grouped by expert: argument block and row-range search
+// shared by the grouped and 4-bit kernels.
+#pragma once
+
+#include "common.h"
+
+namespace pdmb {
+
+// Rows of group e: [ends[e-1], ends[e]) of the T activation rows (ends[-1] = 0).
+// kind kRows:   C[r] = A[r] @ B[e]           A [T,K] (lda), B[e] at e * sB, C [T,N] (ldc)
+// kind kReduce: C[e] = A_e^T @ B_e           A [T,M] (lda), B [T,N] (ldb), C[e] [M,N] at e * sC
+// Strides in elements.
+struct GroupArgs {
+  const void* A;
+  const void* B;
+  void* C;
+  const void* ends;  // E running ends, int32 or (ends64) int64
+  int ends64;
+  int E, T;
+  int M, N, K;       // kRows: N, K; kReduce: M, N
+  long long lda, ldb, ldc, sB, sC;
+  int tiles_m, tiles_n;  // kReduce: tiles of one C[e]; kRows: tiles_n
+  int zero_tail;     // kRows: write zeros to the rows behind the last group
+};
+
+// End of group e, held inside [0, T] so that no value of `ends` addresses
+// memory outside the operands (-1 is the start of group 0).
+__device__ __forceinline__ int group_end(const void* ends, int ends64, int T, int e) {
+  if (e < 0) return 0;
+  const long long v = ends64 ? ((const long long*)ends)[e] : (long long)((const int*)ends)[e];
+  return (int)(v < 0 ? 0 : v > T ? T : v);
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over 64 lanes
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d);
+    v += lane >= d ? o : 0;
+  }
+  return v;
+}
+
+// One BM-row tile of a group (e == E: the rows behind the last group).
+struct RowTile {
+  int e, row0, rows;  // first row, rows of it in this tile (1 .. BM)
+};
+
+// Tiles of BM rows of groups [c0, c0 + 64), one group a lane: first row and
+// row count of lane's group, and its tile count.
+template <int BM>
+__device__ __forceinline__ int lane_tiles(const GroupArgs& a, int e, int& lo, int& n) {
+  lo = 0;
+  n = 0;
+  if (e < a.E || (e == a.E && a.zero_tail)) {
+    lo = group_end(a.ends, a.ends64, a.T, e - 1);
+    const int hi = e < a.E ? group_end(a.ends, a.ends64, a.T, e) : a.T;
+    n = hi > lo ? hi - lo : 0;
+  }
+  return (n + BM - 1) / BM;
+}
+
+// The group's tile that L of the launch's row-tile x column-tile products
+// falls to. Every wave of the workgroup searches by itself (no barrier): a
+// lane takes a group, a 64-lane prefix sum gives the tiles before it; more
+// than 64 groups go by 64 a pass. Returns false where block b has no tile.
+//
+// Order: products are dealt to the XCDs (blocks b and b + 8 share one) in
+// runs of up to 32, so that an XCD's 32 CUs work on 8 row tiles x 4 column
+// tiles and its L2 serves each operand panel to several of them.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int lane, RowTile& r, int& tn) {
+  int lo, n;
+  int t = lane_tiles<BM>(a, lane, lo, n);
+  int inc = wave_scan(t, lane);
+  int total = __builtin_amdgcn_readlane(inc, 63);
+  const int groups = a.E + 1;  // the tail counts as one
+  if (groups > 64) {
+    for (int c0 = 64; c0 < groups; c0 += 64) {
+      int lo2, n2;
+      total += __builtin_amdgcn_readlane(wave_scan(lane_tiles<BM>(a, c0 + lane, lo2, n2), lane), 63);
+    }
+  }
+  // XCD-run order over `total` x tiles_n products
+  const unsigned prods = (unsigned)total * (unsigned)a.tiles_n;
+  const unsigned per = (prods + 7) / 8, x = b & 7, i = b >> 3;
+  if (i >= per) return false;
+  const unsigned full = per / 32 * 32;
+  const unsigned L = i < full ? (i / 32) * 256 + x * 32 + i % 32 : full * 8 + x * (per - full) + (i - full);
+  if (L >= prods) return false;
+  const unsigned sg = L / (8u * a.tiles_n), s0 = sg * 8;
+  const unsigned gm = min(8u, (unsigned)total - s0), rem = L - sg * 8u * a.tiles_n;
+  tn = (int)(rem / gm);
+  const int slot = (int)(s0 + rem % gm);
+  int base = 0, c0 = 0;
+  for (;;) {
+    const int tot = __builtin_amdgcn_readlane(inc, 63);
+    if (slot < base + tot) break;
+    base += tot;
+    c0 += 64;
+    t = lane_tiles<BM>(a, c0 + lane, lo, n);
+    inc = wave_scan(t, lane);
+  }
+  const unsigned long long at = __ballot(slot < base + inc);  // first lane whose tiles reach slot
+  const int l = __builtin_ctzll(at);
+  const int before = base + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(t, l);
+  const int off = (slot - before) * BM;
+  r.e = c0 + l;
+  r.row0 = __builtin_amdgcn_readlane(lo, l) + off;
+  r.rows = min(BM, __builtin_amdgcn_readlane(n, l) - off);
+  return true;
+}
+
+// Row tiles that a launch has to provide for: every group may end in a part
+// of a tile, and so may the rows behind the last one.
+inline long long row_tiles_bound(int T, int E, int BM, bool tail) {
+  const long long g = (long long)E + (tail ? 1 : 0);
+  return (long long)T / BM + (g < T ? g : T);
+}
+
+}  // namespace pdmb

@@ -1,0 +1,286 @@
+"""Expert-grouped products on the GPU against 64-bit loops over the experts.
+
+Tolerances: a sum of n fp32 terms is off by at most (n + 2) steps (2^-23 relative,
+whichever way the matrix unit rounds) of the sum of magnitudes; the result's one
+rounding adds half a step of its type, and in fp16 half the smallest
+subnormal, 2^-25."""
+import pytest
+import torch
+
+from pytorch_distributed_matmul_benchmark_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _ends(sizes, dtype=torch.int32):
+    return torch.tensor(sizes).cumsum(0).to(dtype).cuda()
+
+
+def _close(got, exact, magnitude, n):
+    eps = torch.finfo(got.dtype).eps / 2
+    bound = eps * exact.abs() * 1.01 + (n + 2) * 2.0 ** -23 * magnitude + 2.0 ** -25
+    off = (got.double() - exact).abs()
+    assert bool((off <= bound).all()), f"off by {(off / bound).max().item():.3g} of the bound"
+
+
+def _rows_exact(x, w, ends):
+    y = torch.zeros(x.shape[0], w.shape[2], dtype=torch.float64, device="cuda")
+    lo = 0
+    for e, hi in enumerate(ends.tolist()):
+        if hi > lo:
+            y[lo:hi] = x[lo:hi].double() @ w[e].double()
+        lo = hi
+    return y
+
+
+def _reduce_exact(x, dy, ends):
+    w = torch.zeros(len(ends), x.shape[1], dy.shape[1], dtype=torch.float64, device="cuda")
+    lo = 0
+    for e, hi in enumerate(ends.tolist()):
+        w[e] = x[lo:hi].double().t() @ dy[lo:hi].double()
+        lo = hi
+    return w
+
+
+def _data(T, K, N, E, dtype, colmajor=False, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + T * 7 + K)
+    x = torch.randn(T, K, device="cuda", generator=g).to(dtype)
+    w = torch.randn(E, N, K, device="cuda", generator=g) if colmajor else torch.randn(E, K, N, device="cuda", generator=g)
+    w = (w * K ** -0.5).to(dtype)
+    return x, (w.transpose(1, 2) if colmajor else w)
+
+
+# (rows of each expert, rows behind the last, K, N)
+SHAPES = [
+    ([1], 0, 1, 1),
+    ([1], 0, 64, 128),
+    ([3, 0, 2], 0, 8, 8),
+    ([0, 0, 5], 3, 33, 17),            # odd widths, empty experts first
+    ([16, 1, 15, 17], 0, 96, 136),
+    ([40, 31, 0, 33, 64], 7, 200, 264),
+    ([130, 0, 257, 1], 0, 264, 392),
+    ([300, 511, 129], 40, 1000, 520),
+    ([1] * 70, 0, 128, 144),           # more experts than a wave has lanes
+    ([0] * 100 + [9] + [0] * 40, 2, 72, 40),
+    ([700, 900], 0, 512, 512),
+    ([513, 256, 300, 1024], 11, 328, 776),
+    ([600, 0, 700], 0, 257, 300),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"E{len(s[0])}T{sum(s[0])}K{s[2]}N{s[3]}")
+@pytest.mark.parametrize("colmajor", [False, True], ids=["row", "col"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_rows(dtype, colmajor, shape):
+    sizes, behind, K, N = shape
+    x, w = _data(sum(sizes) + behind, K, N, len(sizes), DT[dtype], colmajor)
+    ends = _ends(sizes, torch.int64 if colmajor else torch.int32)
+    y = ops.grouped_matmul(x, w, ends)
+    _close(y, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
+    assert bool((y[sum(sizes):] == 0).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"E{len(s[0])}T{sum(s[0])}K{s[2]}N{s[3]}")
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_reduce(dtype, shape):
+    sizes, behind, K, N = shape
+    x, _ = _data(sum(sizes) + behind, K, 1, 1, DT[dtype])
+    dy, _ = _data(sum(sizes) + behind, N, 1, 1, DT[dtype], seed=5)
+    ends = _ends(sizes)
+    dw = ops.grouped_weight_grad(x, dy, ends)
+    _close(dw, _reduce_exact(x, dy, ends), _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("sizes,K,N", [([5, 0, 9], 40, 72), ([300, 260, 0, 400], 328, 264)])
+def test_views_and_what_lies_beside_them(dtype, sizes, K, N):
+    """Strided views whose neighbours are NaN; NaN in the rows behind the last expert and in the
+    weights of an expert without rows: none of it reaches a result."""
+    dt, T, E = DT[dtype], sum(sizes) + 3, len(sizes)
+    x0, w0 = _data(T, K, N, E, dt)
+    dy0, _ = _data(T, N, 1, 1, dt, seed=3)
+    xb = torch.full((T + 2, K + 24), float("nan"), device="cuda", dtype=dt)
+    wb = torch.full((E, K + 3, N + 8), float("nan"), device="cuda", dtype=dt)
+    db = torch.full((T + 1, N + 7), float("nan"), device="cuda", dtype=dt)
+    for ox, oy in ((8, 0), (3, 1)):  # aligned and not
+        x, w, dy = xb[1:T + 1, ox:ox + K], wb[:, 1:K + 1, oy:oy + N], db[:T, oy:oy + N]
+        x.copy_(x0), w.copy_(w0), dy.copy_(dy0)
+        ends = _ends(sizes)
+        x[T - 3:] = float("nan")
+        dy[T - 3:] = float("inf")
+        w[sizes.index(0)] = float("nan")
+        out = torch.full((T, N + 5), 3.0, device="cuda", dtype=dt)[:, 2:N + 2]
+        base = out.clone()
+        y = ops.grouped_matmul(x, w, ends, out=out)
+        assert y is out and torch.equal(out[T - 3:], base[T - 3:])
+        _close(out[:T - 3], _rows_exact(x0, w0, ends)[:T - 3], _rows_exact(x0.abs(), w0.abs(), ends)[:T - 3], K)
+        dx = ops.grouped_matmul(dy, w.transpose(1, 2), ends)
+        _close(dx, _rows_exact(dy0, w0.transpose(1, 2), ends),
+               _rows_exact(dy0.abs(), w0.transpose(1, 2).abs(), ends), N)
+        dw = ops.grouped_weight_grad(x, dy, ends)
+        _close(dw, _reduce_exact(x0, dy0, ends), _reduce_exact(x0.abs(), dy0.abs(), ends), max(sizes))
+        wb.fill_(float("nan")), xb.fill_(float("nan")), db.fill_(float("nan"))
+
+
+def test_infinities_stay_in_their_rows():
+    x, w = _data(600, 256, 256, 2, torch.bfloat16)
+    ends = _ends([300, 300])
+    clean = ops.grouped_matmul(x, w, ends)
+    x[17, 5] = float("inf")
+    x[400, 255] = float("nan")
+    y = ops.grouped_matmul(x, w, ends)
+    keep = torch.ones(600, dtype=torch.bool, device="cuda")
+    keep[17] = keep[400] = False
+    assert torch.equal(y[keep], clean[keep])
+    assert not bool(y[17].isfinite().any()) and bool(y[400].isnan().all())
+
+
+def test_empty_sizes():
+    w = torch.randn(2, 16, 8, device="cuda")
+    z = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert ops.grouped_matmul(torch.zeros(0, 16, device="cuda"), w, z).shape == (0, 8)
+    assert bool((ops.grouped_matmul(torch.ones(3, 16, device="cuda"), w, z) == 0).all())
+    assert bool((ops.grouped_matmul(torch.ones(3, 0, device="cuda"), w[:, :0], z + 3) == 0).all())
+    assert ops.grouped_matmul(torch.ones(3, 16, device="cuda"), w[:, :, :0], z + 3).shape == (3, 0)
+    assert bool((ops.grouped_weight_grad(torch.zeros(0, 16, device="cuda"), torch.zeros(0, 8, device="cuda"), z) == 0).all())
+
+
+def test_ends_outside_the_rows_are_held_inside():
+    x, w = _data(40, 64, 64, 3, torch.bfloat16)
+    y = ops.grouped_matmul(x, w, torch.tensor([-7, 25, 10 ** 6], device="cuda"))
+    assert torch.equal(y, ops.grouped_matmul(x, w, _ends([0, 25, 15])))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("colmajor", [False, True], ids=["row", "col"])
+@pytest.mark.parametrize("sizes,K,N", [([9, 0, 30, 1], 72, 40), ([300, 513, 0, 260], 256, 512)])
+def test_gradients(dtype, colmajor, sizes, K, N):
+    dt = DT[dtype]
+    x, w = _data(sum(sizes) + 4, K, N, len(sizes), dt, colmajor)
+    dy, _ = _data(sum(sizes) + 4, N, 1, 1, dt, seed=9)
+    ends = _ends(sizes)
+    x.requires_grad_(), w.requires_grad_()
+    y = ops.native_grouped_matmul(x, w, ends)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x, w = x.detach(), w.detach()
+    assert dw.stride() == w.stride()
+    _close(dx, _rows_exact(dy, w.transpose(1, 2), ends), _rows_exact(dy.abs(), w.transpose(1, 2).abs(), ends), N)
+    _close(dw, _reduce_exact(x, dy, ends), _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
+    # against differences of the product itself, which is linear in each factor: twice the bound
+    # of a sum over all outputs, each within half a step and (K + 2) fp32 steps
+    d, _ = _data(sum(sizes) + 4, K, 1, 1, dt, seed=21)
+    with torch.no_grad():
+        f = ops.grouped_matmul(d, w, ends).double()
+        mag = _rows_exact(d.abs(), w.abs(), ends)
+    eps = torch.finfo(dt).eps / 2 + (K + N + 4) * 2.0 ** -23
+    slack = 2 * eps * (mag * dy.double().abs()).sum()
+    assert abs((dx.double() * d.double()).sum() - (f * dy.double()).sum()) <= slack
+
+
+def test_only_the_gradients_asked_for():
+    x, w = _data(20, 32, 16, 2, torch.bfloat16)
+    ends = _ends([9, 11])
+    (dx,) = torch.autograd.grad(ops.native_grouped_matmul(x.requires_grad_(), w, ends).sum(), x)
+    (dw,) = torch.autograd.grad(ops.native_grouped_matmul(x.detach(), w.requires_grad_(), ends).sum(), w)
+    assert dx.shape == x.shape and dw.shape == w.shape
+
+
+def test_other_stream():
+    x, w = _data(500, 512, 512, 4, torch.bfloat16)
+    ends = _ends([100, 200, 0, 200])
+    want = ops.grouped_matmul(x, w, ends)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.grouped_matmul(x, w, ends)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T,K,N,E", [(64, 256, 256, 8), (1500, 512, 512, 4)])
+def test_captured_graph_follows_the_sizes(T, K, N, E):
+    x, w = _data(T, K, N, E, torch.bfloat16)
+    dy, _ = _data(T, N, 1, 1, torch.bfloat16, seed=2)
+    ends = torch.empty(E, dtype=torch.int32, device="cuda")
+    plans = [[T // E] * E, [T] + [0] * (E - 1), [0] * (E - 1) + [T - 3], [1] * E]
+    ends.copy_(_ends(plans[0]))
+    for _ in range(2):
+        ops.grouped_matmul(x, w, ends), ops.grouped_weight_grad(x, dy, ends)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.grouped_matmul(x, w, ends)
+        dx = ops.grouped_matmul(dy, w.transpose(1, 2), ends)
+        dw = ops.grouped_weight_grad(x, dy, ends)
+    for sizes in plans * 2:
+        ends.copy_(_ends(sizes))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.grouped_matmul(x, w, ends))
+        assert torch.equal(dx, ops.grouped_matmul(dy, w.transpose(1, 2), ends))
+        assert torch.equal(dw, ops.grouped_weight_grad(x, dy, ends))
+
+
+def test_repeats_bit_for_bit():
+    x, w = _data(1000, 768, 640, 6, torch.bfloat16)
+    ends = _ends([10, 500, 0, 90, 300, 100])
+    dy, _ = _data(1000, 640, 1, 1, torch.bfloat16, seed=2)
+    y, dw = ops.grouped_matmul(x, w, ends), ops.grouped_weight_grad(x, dy, ends)
+    for _ in range(5):
+        assert torch.equal(y, ops.grouped_matmul(x, w, ends))
+        assert torch.equal(dw, ops.grouped_weight_grad(x, dy, ends))
+
+
+def test_refusals_on_the_gpu():
+    x, w, ends = torch.zeros(4, 32, device="cuda"), torch.zeros(2, 32, 8, device="cuda"), _ends([1, 3])
+    with pytest.raises(ValueError):
+        ops.grouped_matmul(x, w, ends.cpu())
+    with pytest.raises(ValueError):
+        ops.grouped_matmul(x, w.cpu(), ends)
+    with pytest.raises(ValueError):
+        ops.grouped_weight_grad(x, torch.zeros(4, 8), ends)
+    with pytest.raises(RuntimeError):  # overlapping rows of out
+        ops.grouped_matmul(x, w, ends, out=torch.zeros(1, 8, device="cuda").expand(4, 8))
+
+
+def _mlp(x, ends, up, down, product):
+    h = product(x, up, ends)
+    return product(torch.nn.functional.silu(h), down, ends)
+
+
+def test_an_expert_layer_trained_and_served():
+    """The operators as they are used together: rows routed to experts, ordered, through two grouped
+    products and back, with gradients; then the same layer with 4-bit experts, token by token."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tokens, wide, hidden, E = 200, 256, 384, 8
+    x = torch.randn(tokens, wide, device="cuda", generator=g)
+    up = (torch.randn(E, wide, hidden, device="cuda", generator=g) / 16).requires_grad_()
+    down = (torch.randn(E, hidden, wide, device="cuda", generator=g) / 16).requires_grad_()
+    who = torch.randint(0, E, (tokens,), device="cuda", generator=g)
+    order = torch.argsort(who, stable=True)
+    ends = torch.bincount(who, minlength=E).cumsum(0)
+    y = torch.empty_like(x).index_put((order,), _mlp(x[order], ends, up, down, ops.native_grouped_matmul))
+    grads = torch.autograd.grad(y.square().sum(), (up, down))
+
+    upd, downd = up.detach().double().requires_grad_(), down.detach().double().requires_grad_()
+    rows = [torch.nn.functional.silu(x[t].double() @ upd[who[t]]) @ downd[who[t]] for t in range(tokens)]
+    ref = torch.stack(rows)
+    want = torch.autograd.grad(ref.square().sum(), (upd, downd))
+    # two products of 256 and 384 terms in fp32 and the silu between them
+    assert ((y.double() - ref).norm() / ref.norm()).item() < (256 + 384 + 8) * 2.0 ** -24
+    for a, b in zip(grads, want):
+        assert ((a.double() - b).norm() / b.norm()).item() < 4 * (256 + 384 + 8) * 2.0 ** -24
+
+    packed = [ops.int4_quantize(p.detach().bfloat16(), 64) for p in (up, down)]
+    plain = [ops.int4_dequantize(*p).double() for p in packed]
+    xb = x.bfloat16()
+    for t in range(0, tokens, 37):  # one token a step
+        one = (torch.arange(E, device="cuda") >= who[t]).to(torch.int32)
+        h = ops.int4_matmul(xb[t:t + 1], *packed[0], ends=one)
+        out = ops.int4_matmul(torch.nn.functional.silu(h), *packed[1], ends=one)
+        a = xb[t].double() @ plain[0][who[t]]
+        ref = torch.nn.functional.silu(a) @ plain[1][who[t]]
+        # bf16 roundings: of h, of silu(h) (its slope is below 1.1) and of the result
+        assert ((out[0].double() - ref).norm() / ref.norm()).item() < 3.3 * 2.0 ** -8
