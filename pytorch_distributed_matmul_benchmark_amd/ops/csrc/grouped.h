@@ -117,4 +117,9 @@ inline long long row_tiles_bound(int T, int E, int BM, bool tail) {
   return (long long)T / BM + (g < T ? g : T);
 }
 
+// The large-tile kernel of 16-bit products (grouped_w4.hip): whether its loads
+// and offsets fit the problem, and its launch.
+bool grouped_w4_ok(const GroupArgs& a, bool red, bool colmajor);
+hipError_t grouped_w4(const GroupArgs& a, int dtype, bool red, bool colmajor, hipStream_t s);
+
 }  // namespace pdmb

@@ -325,6 +325,10 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
   const bool c_ok = (uintptr_t)p.C % (4 * es) == 0 && p.ldc % 4 == 0 && p.sC % 4 == 0;
   const bool vec = c_ok && vec_ok(p.A, p.lda, 0, es, red ? p.M : p.K) &&
                    vec_ok(p.B, p.ldb, p.sB, es, red || !p.b_colmajor ? p.N : p.K);
+  const int avg = (p.T + p.E - 1) / p.E;
+  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 192) && (red || p.K > 0) &&
+      grouped_w4_ok(a, red, p.b_colmajor))
+    return grouped_w4(a, p.dtype, red, p.b_colmajor, stream);
   switch (p.dtype) {
     case kF32:
       return red            ? kgrp::launch_reduce<kF32>(a, vec, stream)
