@@ -216,9 +216,11 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream);
 // Products with 4-bit weights and group scales (int4.hip), 16-bit X and C:
 //   C[r] = X[r] @ W[e]^T,  W[e][n][k] = scale[e][n][k / G] * (q[e][n][k] - zero[e][n][k / G])
 // q holds two values a byte, even k in the low half: [N, K/2] bytes, 16-B aligned
-// rows of K/2; scale [N, K/G] in X's type, zero [N, K/G] bytes (nullptr: 8), both
-// contiguous, per group [E]. ends == nullptr: one group that owns all T rows;
-// otherwise as for GroupedProblem. K % G == 0, G % 32 == 0.
+// rows of K/2; scale [N, K/G] in X's type, zero [N, K/G] bytes (their low
+// four bits; nullptr: 8), both
+// contiguous, per group [E]. X rows 16-B aligned. ends == nullptr: one group that
+// owns all T rows; otherwise as for GroupedProblem. K % G == 0; G is 32, 64 or a
+// multiple of 128.
 struct Int4Problem {
   int dtype;
   const void* X;

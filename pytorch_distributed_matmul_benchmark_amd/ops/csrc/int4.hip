@@ -4,21 +4,30 @@
 // of rows.
 //
 // Exactness: the nibbles go into the matrix instructions as whole numbers, so
-// a weight is never rounded: bits of 16 + q are formed by one shift and one
-// and-or for two values (16 .. 31 have the step 1 at a fixed mantissa place:
-// bf16 0x4180 | q << 3, fp16 0x4c00 | q << 6). fp16 subtracts 16 + zero
-// exactly (v_pk_add_f16); bf16, which has no packed add, adds a second product with the
-// constant -(16 + zero), also a whole number, to the same fp32 sum. Each
-// group's fp32 sum is scaled once, in fp32. (A row of X with an infinity
-// gives NaN in bf16: the two products cancel.)
+// a weight is never rounded. Two values at a time, at one place of a dword's
+// halves, become B + q (a power of two B whose mantissa step fits the place) by
+// one and-or, most after one shift:
+//   bf16  B = 128 for nibble 0 (bits 0-3 as they are), 16 for the others (shifted to bits 3-6)
+//   fp16  B = 1024: nibbles 0 and 2 at bits 0-3, 1 and 3 at bits 4-7 (16 times the value)
+// fp16 then subtracts B + zero exactly (v_pk_add_f16, for bits 4-7 v_pk_fma_f16 with
+// 1/16); bf16, which has no packed add, adds a second product with the constants
+// -(B + zero), also whole numbers, to the same fp32 sum. Each group's fp32 sum is
+// scaled once, in fp32. (A row of X with an infinity gives NaN in bf16: the two
+// products cancel.)
 //
-// A wave takes 16 NB columns and every W-th chunk of 128 k: lane (l16, g)
-// loads 16 bytes (32 nibbles) of column l16 at byte 16 g of its 64-byte run.
-// Four dwords a lane are transposed among the four 16-lane rows (two
-// v_permlane32_swap, two v_permlane16_swap) so that the lane's dword j holds k
-// 32 j + 8 g .. + 7: MFMA j then covers 32 consecutive k, the smallest group.
-// A dword's halves hold nibbles i and i + 4; the row fragments are permuted
-// the same way. The W waves' sums meet in LDS, added in wave order.
+// Loads: an MFMA operand has its 16 columns in neighbouring lanes, but 16-byte
+// loads whose neighbours are in 16 rows of memory look a cache line up for
+// every lane (measured: 13 bytes a ns and CU whatever the tile, depth or number of
+// waves). So four lanes load 64 bytes of one column, 128 k, and
+// ds_bpermute brings each dword to the operand's lane (l16, g): 16 bytes, k 32 g ..
+// + 31. Its four dwords are then transposed among the four 16-lane rows (two
+// v_permlane32_swap, two v_permlane16_swap): dword j holds k 32 j + 8 g .. + 7,
+// and MFMA j covers 32 consecutive k, the smallest group. A dword's halves hold
+// nibbles i and i + 4; the rows' fragments are permuted the same way on their way
+// through LDS ([row][256 B], 16-B piece c at c ^ row: conflict-free both ways).
+//
+// Two kernels: gemm_int4_few for up to 16 rows of a weight, bound by the read of the
+// weight, and gemm_int4_rows for more, where the rows come through LDS.
 #include "api.h"
 #include "grouped.h"
 
@@ -29,8 +38,14 @@ struct Args : GroupArgs {
   const void* scale;
   const unsigned char* zero;
   int groups;   // K / G
-  int chunk_g;  // 128-k chunks of one group (G >= 128), else 1
+  unsigned chunk_g;  // G > 128: ceil(2^32 / (G / 128)), else 0
 };
+
+// Group of chunk c where a group is one chunk or more. (c and G / 128 are at most K / 128
+// <= 2^16, so the product with the rounded-up reciprocal is exact.)
+__device__ __forceinline__ int group_of(const Args& a, int c) {
+  return a.chunk_g ? (int)__umulhi((unsigned)c, a.chunk_g) : c;
+}
 
 // {r0, r1, r2, r3} of lane row g -> dword g of lane rows 0 .. 3
 __device__ __forceinline__ void transpose4(u32x4& r) {
@@ -48,35 +63,228 @@ __device__ __forceinline__ s16x8 permute_row(const u32x4& x) {
   return __builtin_bit_cast(s16x8, v);
 }
 
-// 8 nibbles as 16 + q (bf16) or q - zero (fp16; minus = -(16 + zero) twice)
+// The and-or constants in registers (an instruction that does both takes no literal).
+struct Bits {
+  unsigned mask0, mask1, or0, or1;
+  template <int DT>
+  __device__ static __forceinline__ Bits make() {
+    Bits b = DT == kBF16 ? Bits{0x000f000fu, 0x00780078u, 0x43004300u, 0x41804180u}
+                         : Bits{0x000f000fu, 0x00f000f0u, 0x64006400u, 0x64006400u};
+    asm("" : "+s"(b.mask0), "+s"(b.mask1), "+v"(b.or0), "+v"(b.or1));
+    return b;
+  }
+};
+
+// What widen() subtracts for a zero point, two halves each: [0] -(B + zero) of the first pair,
+// [1] of the others. fp16: [1] -(64 + zero), after the 1/16.
+struct Minus {
+  unsigned m[2];
+};
 template <int DT>
-__device__ __forceinline__ s16x8 widen(unsigned d, unsigned minus) {
+__device__ __forceinline__ Minus minus_of(unsigned z) {
+  // (bf16 128 + z: step 1 at bit 0, 16 + z: bit 3; fp16 1024 + z: bit 0, 64 + z: bit 4)
+  return DT == kBF16 ? Minus{{z * 0x00010001u + 0xc300c300u, z * 0x00080008u + 0xc180c180u}}
+                     : Minus{{z * 0x00010001u + 0xe400e400u, z * 0x00100010u + 0xd400d400u}};
+}
+
+// 8 nibbles as B + q (bf16; EVEN: B = 16 for all), or as q - zero (fp16).
+template <int DT, bool EVEN = false>
+__device__ __forceinline__ s16x8 widen(unsigned d, const Bits& b, const Minus& minus) {
   u32x4 v;
   if constexpr (DT == kBF16) {
-    v = u32x4{((d << 3) & 0x00780078u) | 0x41804180u, ((d >> 1) & 0x00780078u) | 0x41804180u,
-              ((d >> 5) & 0x00780078u) | 0x41804180u, ((d >> 9) & 0x00780078u) | 0x41804180u};
+    v = u32x4{EVEN ? ((d << 3) & b.mask1) | b.or1 : (d & b.mask0) | b.or0, ((d >> 1) & b.mask1) | b.or1, ((d >> 5) & b.mask1) | b.or1,
+              ((d >> 9) & b.mask1) | b.or1};
   } else {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 m = __builtin_bit_cast(f16x2, minus);
-    v = u32x4{((d << 6) & 0x03c003c0u) | 0x4c004c00u, ((d << 2) & 0x03c003c0u) | 0x4c004c00u,
-              ((d >> 2) & 0x03c003c0u) | 0x4c004c00u, ((d >> 6) & 0x03c003c0u) | 0x4c004c00u};
+    const f16x2 m0 = __builtin_bit_cast(f16x2, minus.m[0]), m1 = __builtin_bit_cast(f16x2, minus.m[1]);
+    const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const unsigned e = d >> 8;
+    const f16x2 w[4] = {__builtin_bit_cast(f16x2, (d & b.mask0) | b.or0) + m0,
+                        __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (d & b.mask1) | b.or1), sixteenth, m1),
+                        __builtin_bit_cast(f16x2, (e & b.mask0) | b.or0) + m0,
+                        __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (e & b.mask1) | b.or1), sixteenth, m1)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, (unsigned)v[i]) + m);
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(unsigned, w[i]);
   }
   return __builtin_bit_cast(s16x8, v);
 }
 
-// SG: scales of a 128-k chunk (G = 32: 4, 64: 2, 128 and more: 1).
-template <int MB, int NB, int SG>
-struct Stage {
-  u32x4 q[NB], x[MB][4];
-  unsigned short s[NB][SG];
-  unsigned char z[NB][SG];
+// G = 32: SG = 4 scales and zero points a chunk of 128 k, 64: 2, 128 and more: 1.
+// Scales and zero points of C neighbouring chunks of one column, as loaded; ZERO:
+// zero points are given (otherwise 8).
+template <int BYTES>
+struct Raw {  // BYTES from any address in as few loads as there are dwords
+  unsigned w[(BYTES + 3) / 4];
+  __device__ __forceinline__ void load(const void* p) {
+    if constexpr (BYTES == 1) w[0] = *(const unsigned char*)p;
+    else if constexpr (BYTES == 2) { unsigned short v; __builtin_memcpy(&v, p, 2); w[0] = v; }
+    else __builtin_memcpy(w, p, BYTES);
+  }
+  __device__ __forceinline__ unsigned half(int i) const { return i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu; }
+  __device__ __forceinline__ unsigned byte(int i) const { return (w[i >> 2] >> (8 * (i & 3))) & 255u; }
+};
+template <int DT, int SG, int C, bool ZERO>
+struct Scales {
+  static constexpr int N = SG * C;
+  Raw<2 * N> s;
+  Raw<N> z;
+  __device__ __forceinline__ void load(const unsigned short* sp, const unsigned char* zp) {
+    s.load(sp);
+    if constexpr (ZERO) z.load(zp);
+  }
+  __device__ __forceinline__ void load_lds(const char* sp, const char* zp) {
+    typedef __attribute__((address_space(3))) unsigned lds_u32;
+    typedef __attribute__((address_space(3))) unsigned short lds_u16;
+    typedef __attribute__((address_space(3))) unsigned char lds_u8;
+    static_assert(C == 1, "one chunk");
+    if constexpr (SG == 1) {
+      s.w[0] = *(const lds_u16*)sp;
+      if constexpr (ZERO) z.w[0] = *(const lds_u8*)zp;
+    } else if constexpr (SG == 2) {
+      s.w[0] = *(const lds_u32*)sp;
+      if constexpr (ZERO) z.w[0] = *(const lds_u16*)zp;
+    } else {
+      const u32x2 v = *(const lds_u32x2*)sp;
+      s.w[0] = v.x;
+      s.w[1] = v.y;
+      if constexpr (ZERO) z.w[0] = *(const lds_u32*)zp;
+    }
+  }
+  // one by one, the last group repeated: what is left of a column
+  __device__ __forceinline__ void load_part(const unsigned short* sp, const unsigned char* zp, int groups) {
+#pragma unroll
+    for (int t = 0; t < (2 * N + 3) / 4; ++t) s.w[t] = 0;
+#pragma unroll
+    for (int t = 0; t < (N + 3) / 4; ++t) z.w[t] = 0;
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      s.w[t >> 1] |= (unsigned)sp[min(t, groups - 1)] << (16 * (t & 1));
+      if constexpr (ZERO) z.w[t >> 2] |= (unsigned)zp[min(t, groups - 1)] << (8 * (t & 3));
+    }
+  }
+  __device__ __forceinline__ float scale(int t) const {
+    if constexpr (DT == kBF16) return __uint_as_float(t & 1 ? s.w[t >> 1] & 0xffff0000u : s.w[t >> 1] << 16);
+    else return to_f32<DT>((unsigned short)s.half(t));
+  }
+  __device__ __forceinline__ unsigned zero(int t) const { return ZERO ? z.byte(t) & 15u : 8u; }
 };
 
-template <int DT, int MB, int NB, int SG, int W>
-__global__ void __launch_bounds__(64 * W) gemm_int4(Args a) {
-  __shared__ float red[W][MB * NB * 4 * 64];
+// A lane's columns. Loads: column 16 j + (lane >> 2), 16-B piece lane & 3. Scales:
+// column 16 j + l16.
+template <int NB>
+struct Columns {
+  const unsigned char* q[NB];
+  const unsigned short* s[NB];
+  const unsigned char* z[NB];
+  __device__ __forceinline__ Columns(const Args& a, int e, int n0, int lane) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const long long base = (long long)e * a.N;
+      const long long nq = base + min(n0 + 16 * j + (lane >> 2), a.N - 1);
+      const long long ns = base + min(n0 + 16 * j + (lane & 15), a.N - 1);
+      q[j] = (const unsigned char*)a.B + nq * (a.K / 2) + 16 * (lane & 3);
+      s[j] = (const unsigned short*)a.scale + ns * a.groups;
+      z[j] = a.zero + ns * a.groups;
+    }
+  }
+};
+
+// As loaded -> the operand's lanes (column l16, k 32 j + 8 g .. + 7 in dword j).
+__device__ __forceinline__ void to_operand(u32x4& v, int from) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)v[i]);
+  transpose4(v);
+}
+
+// The tile's rows as a buffer whose range ends with the last row: offsets of
+// rows (or k) that there are not go past it and read as zeros, with no branch.
+constexpr int kOutside = (int)0x80000000;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const Args& a, const RowTile& r) {
+  return __builtin_amdgcn_make_buffer_rsrc((char*)a.A + (long long)r.row0 * a.lda * 2, 0,
+                                           (int)(((long long)(r.rows - 1) * a.lda + a.K) * 2), 0x00020000);
+}
+__device__ __forceinline__ u32x4 load_row(__amdgpu_buffer_rsrc_t x, int off, int soff) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(x, off, soff, 0));
+}
+
+// ---- up to 16 rows -------------------------------------------------------
+// A workgroup takes 16 NB columns, its W waves a run of k each, one chunk of 128 k a
+// step with the next D in flight; each wave passes its part of the rows (4 RX
+// of them) through LDS of its own. The W sums meet in LDS, added in wave order.
+//
+// Scales and zero points of KB chunks at a time go to LDS first, 8 groups a
+// lane: read where they are used they cost a cache line look-up for every
+// lane (a 16 x 4096 x 11007 product with groups of 32: 128 of a chunk's 208).
+//
+// The loop has no branches around loads (a conditional load makes hipcc wait for
+// the loads after it as well): chunk numbers past the end repeat the last one and
+// are not computed; a partial last chunk reads weights from inside the column
+// and zeros for the rows.
+constexpr int KB = 64;
+
+template <int NB, int SG>
+struct ScaleBlock {  // [column][KB * SG groups], 8 bytes between columns against bank conflicts
+  static constexpr int NG = KB * SG, SP = 2 * NG + 8, ZP = NG + 8, BYTES = 16 * NB * (SP + ZP);
+  static constexpr int PIECES = 16 * NB * NG / 8;  // of 8 groups
+};
+
+template <int NB, int RX>
+struct Step {
+  u32x4 q[NB], x[RX];
+};
+
+template <int DT, int NB, int SG, int RX, bool ZERO>
+__device__ __forceinline__ void multiply(f32x4 (&acc)[NB], Step<NB, RX>& b, const Bits& bits, char* xl, const char* sl,
+                                         int at, int lane) {
+  using SB = ScaleBlock<NB, SG>;
+  constexpr int PER = 4 / SG;  // MFMAs of a group
+  const int l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < RX; ++i) {
+    const int row = 4 * i + g;  // piece l16 of it
+    *(lds_u32x4_t*)(xl + row * 256 + ((l16 ^ row) << 4)) = __builtin_bit_cast(u32x4, permute_row(b.x[i]));
+  }
+  Scales<DT, SG, 1, ZERO> sc[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int c = 16 * j + l16;
+    sc[j].load_lds(sl + c * SB::SP + 2 * at, sl + 16 * NB * SB::SP + c * SB::ZP + at);
+    to_operand(b.q[j], (l16 * 4 + g) * 4);
+  }
+  f32x4 p[NB];
+  Minus minus[NB];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const s16x8 xf = *(const lds_s16x8*)(xl + l16 * 256 + (((4 * t + g) ^ l16) << 4));
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if (t % PER == 0) {
+        minus[j] = minus_of<DT>(sc[j].zero(t / PER));
+        p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      p[j] = mfma16x16x32<DT>(xf, widen<DT>(b.q[j][t], bits, minus[j]), p[j]);
+      if constexpr (DT == kBF16) {
+        const u32x4 m = {minus[j].m[0], minus[j].m[1], minus[j].m[1], minus[j].m[1]};
+        p[j] = mfma16x16x32<DT>(xf, __builtin_bit_cast(s16x8, m), p[j]);
+      }
+    }
+    if (t % PER == PER - 1) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const float s = sc[j].scale(t / PER);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[j][v] = fmaf(s, p[j][v], acc[j][v]);
+      }
+    }
+  }
+}
+
+template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
+__global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
+  using SB = ScaleBlock<NB, SG>;
+  constexpr int XL = 4096, XS = W * (NB > 4 ? NB * 1024 : XL);  // a wave's rows of a chunk; later its sums
+  static_assert(NB <= 4, "the sums reuse the rows' LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[XS + SB::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -84,29 +292,166 @@ __global__ void __launch_bounds__(64 * W) gemm_int4(Args a) {
   RowTile r;
   int tn;
   if (a.ends) {
-    if (!find_tile<16 * MB>(a, blockIdx.x, lane, r, tn)) return;
+    if (!find_tile<16>(a, blockIdx.x, lane, r, tn)) return;
   } else {
     tn = blockIdx.x % a.tiles_n;
     r.e = 0;
-    r.row0 = blockIdx.x / a.tiles_n * (16 * MB);
-    r.rows = min(16 * MB, a.T - r.row0);
+    r.row0 = blockIdx.x / a.tiles_n * 16;
+    r.rows = min(16, a.T - r.row0);
     if (r.rows <= 0) return;
   }
   const int n0 = tn * (16 * NB);
-  const int K = r.e == a.E ? 0 : a.K;  // rows behind the last group: zeros
-  const long long col = (long long)(r.e == a.E ? 0 : r.e) * a.N;
-
-  const unsigned char* qp[NB];
-  const unsigned short* sp[NB];
-  const unsigned char* zp[NB];
+  char* xl = smem + w * XL;
+  char* sl = smem + XS;
+  f32x4 acc[NB];
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const long long n = col + min(n0 + 16 * j + l16, a.N - 1);
-    qp[j] = (const unsigned char*)a.B + n * (a.K / 2) + 16 * g;
-    sp[j] = (const unsigned short*)a.scale + n * a.groups;
-    zp[j] = a.zero + n * a.groups;
+  for (int j = 0; j < NB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int nc = r.e == a.E ? 0 : (a.K + 127) / 128;  // (rows behind the last group: zeros)
+  if (nc > 0) {
+    const int part = a.K % 128;  // k of a partial last chunk
+    const long long first = (long long)r.e * a.N;
+    const unsigned char* q[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      q[j] = (const unsigned char*)a.B + (first + min(n0 + 16 * j + (lane >> 2), a.N - 1)) * (a.K / 2) + 16 * (lane & 3);
+    const __amdgpu_buffer_rsrc_t xr = rows_buffer(a, r);
+    int xo[RX], xt[RX];  // row offsets, and those of the last chunk
+#pragma unroll
+    for (int i = 0; i < RX; ++i) {
+      xo[i] = 4 * i + g < r.rows ? (4 * i + g) * (int)a.lda * 2 + 16 * l16 : kOutside;
+      xt[i] = part && 8 * l16 >= part ? kOutside : xo[i];
+    }
+    const int qt = part ? min(16 * (lane & 3), part / 2 - 16) - 16 * (lane & 3) : 0;
+#pragma unroll
+    for (int i = RX * 4 + g; i < 16; i += 4)  // rows that there are not
+      *(lds_u32x4_t*)(xl + i * 256 + (l16 << 4)) = u32x4{0u, 0u, 0u, 0u};
+    const Bits bits = Bits::make<DT>();
+
+    auto load = [&](Step<NB, RX>& b, int c) {
+      c = min(c, nc - 1);
+      const int at = c * 64 + (c == nc - 1 ? qt : 0);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b.q[j] = *(const u32x4*)(q[j] + at);
+#pragma unroll
+      for (int i = 0; i < RX; ++i) b.x[i] = load_row(xr, c == nc - 1 ? xt[i] : xo[i], c * 256);
+    };
+
+    for (int k0 = 0; k0 < nc; k0 += KB) {
+      const int kn = min(KB, nc - k0), per = (kn + W - 1) / W;
+      const int g0 = SG > 1 ? k0 * SG : group_of(a, k0);
+      int c = k0 + w * per;
+      const int end = min(k0 + kn, c + per);
+      // this block's scales, 8 groups a lane; what is not there is zero
+      constexpr int CH = (SB::PIECES + 64 * W - 1) / (64 * W);
+      u32x4 sv[CH];
+      u32x2 zv[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int at = tid + i * 64 * W, col = at / (SB::NG / 8), gr = g0 + at % (SB::NG / 8) * 8;
+        const long long off = (first + min(n0 + col, a.N - 1)) * a.groups + gr;
+        const unsigned short* sp = (const unsigned short*)a.scale + off;
+        const unsigned char* zp = a.zero + off;
+        sv[i] = u32x4{0u, 0u, 0u, 0u};
+        zv[i] = u32x2{0u, 0u};
+        if (gr + 8 <= a.groups) {
+          __builtin_memcpy(&sv[i], sp, 16);
+          if constexpr (ZERO) __builtin_memcpy(&zv[i], zp, 8);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 7; ++t)
+            if (gr + t < a.groups) {
+              sv[i][t >> 1] |= (unsigned)sp[t] << (16 * (t & 1));
+              if constexpr (ZERO) zv[i][t >> 2] |= (unsigned)zp[t] << (8 * (t & 3));
+            }
+        }
+      }
+      Step<NB, RX> st[D];
+#pragma unroll
+      for (int d = 0; d < D; ++d) load(st[d], c + d);
+      if (k0 > 0) __syncthreads();  // the block before is used up
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int at = tid + i * 64 * W, col = at / (SB::NG / 8), gr = at % (SB::NG / 8) * 8;
+        if (SB::PIECES % (64 * W) == 0 || at < SB::PIECES) {
+          char* p = sl + col * SB::SP + 2 * gr;
+          *(lds_u32x2*)p = u32x2{sv[i][0], sv[i][1]};
+          *(lds_u32x2*)(p + 8) = u32x2{sv[i][2], sv[i][3]};
+          if constexpr (ZERO) *(lds_u32x2*)(sl + 16 * NB * SB::SP + col * SB::ZP + gr) = zv[i];
+        }
+      }
+      __syncthreads();
+      auto mul = [&](Step<NB, RX>& b, int c) {
+        const int at = SG > 1 ? (c - k0) * SG : group_of(a, c) - g0;
+        multiply<DT, NB, SG, RX, ZERO>(acc, b, bits, xl, sl, at, lane);
+      };
+      for (int left = (per + D - 1) / D; left > 1; --left, c += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+          if (c + d < end) mul(st[d], c + d);
+          load(st[d], c + D + d);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+        if (c + d < end) mul(st[d], c + d);
+    }
   }
-  const unsigned short* xp = (const unsigned short*)a.A + ((long long)r.row0 + l16) * a.lda + 8 * g;
+
+  float* red = (float*)smem;  // [wave][16 NB columns x 16 rows]
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) red[w * (NB * 256) + (j * 4 + v) * 64 + lane] = acc[j][v];
+  __syncthreads();
+  for (int at = tid; at < NB * 256; at += 64 * W) {
+    const int ln = at & 63, v = (at >> 6) & 3, j = at >> 8;
+    const int m = 4 * (ln >> 4) + v, n = n0 + j * 16 + (ln & 15);
+    if (m >= r.rows || n >= a.N) continue;
+    float s = red[at];
+#pragma unroll
+    for (int u = 1; u < W; ++u) s += red[u * (NB * 256) + at];
+    ((unsigned short*)a.C)[((long long)r.row0 + m) * a.ldc + n] = (unsigned short)pack2<DT>(s, 0.f);
+  }
+}
+
+// ---- more rows -----------------------------------------------------------
+// A workgroup takes 16 MB rows x 64 NB columns: 4 column waves of 16 NB
+// columns, twice, for the even and the odd chunks of k. The rows of both chunks
+// are staged through LDS, permuted on the way in ([row][256 B], 16-B piece c
+// at c ^ (row & 15): conflict-free both ways), the next pair in registers
+// meanwhile. In bf16 a group's correction (16 + zero) * (sum of x) takes the
+// sum from one product with ones for all of a wave's columns.
+template <int DT, int MB, int NB, int SG, bool ZERO>
+__global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
+  constexpr int BM = 16 * MB, BN = 64 * NB, XB = BM * 256;  // bytes of a chunk's rows
+  constexpr int CH = 2 * XB / 16 / 512;                     // 16-B pieces a thread stages
+  constexpr int RED = 4 * 64 * MB * NB * 4 * 4;
+  constexpr int LDS = 4 * XB > RED ? 4 * XB : RED;
+  static_assert(CH * 512 * 16 == 2 * XB, "whole pieces");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wc = w & 3, half = w >> 2;
+  const int l16 = lane & 15, g = lane >> 4;
+
+  RowTile r;
+  int tn;
+  if (a.ends) {
+    if (!find_tile<BM>(a, blockIdx.x, lane, r, tn)) return;
+  } else {
+    // row tiles of one column tile side by side: the weight is read from memory once
+    const int tm = (a.T + BM - 1) / BM;
+    tn = blockIdx.x / tm;
+    if (tn >= a.tiles_n) return;
+    r.e = 0;
+    r.row0 = blockIdx.x % tm * BM;
+    r.rows = min(BM, a.T - r.row0);
+  }
+  const int n0 = tn * BN + wc * (16 * NB);
+  const int K = r.e == a.E ? 0 : a.K;  // rows behind the last group: zeros
+  const Columns<NB> cols(a, r.e == a.E ? 0 : r.e, n0, lane);
+  const __amdgpu_buffer_rsrc_t xr = rows_buffer(a, r);
 
   f32x4 acc[MB][NB];
 #pragma unroll
@@ -114,108 +459,180 @@ __global__ void __launch_bounds__(64 * W) gemm_int4(Args a) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int nc = (K + 127) / 128;
-  auto load = [&](Stage<MB, NB, SG>& st, int c) {
-    const int k0 = c * 128;
+  const int np = (K + 255) / 256;  // pairs of chunks
+  const Bits bits = Bits::make<DT>();
+  u32x4 xs[CH], q[NB], qn[NB];
+  Scales<DT, SG, 1, ZERO> s[NB], sn[NB];
+  int xo[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int at = tid + i * 512, row = at >> 5;
+    xo[i] = row < r.rows ? (row * (int)a.lda + (at & 31) * 8) * 2 : kOutside;
+  }
+  auto load_rows = [&](int pair) {
+    const int left = K - pair * 256;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      xs[i] = load_row(xr, (tid & 31) * 8 < left ? xo[i] : kOutside, pair * 512);
+  };
+  // (k past the end: any weight, the rows are zero there)
+  auto load_weight = [&](int pair) {
+    const int c = 2 * pair + half, s0 = SG > 1 ? c * SG : group_of(a, c);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      st.q[j] = u32x4{0u, 0u, 0u, 0u};
-      if (k0 + 32 * g < K) st.q[j] = __builtin_nontemporal_load((const u32x4*)(qp[j] + c * 64));
-      const int s0 = SG > 1 ? c * SG : c / a.chunk_g;
+      const int piece = 16 * (lane & 3);
+      qn[j] = *(const u32x4*)(cols.q[j] - piece + min(c * 64 + piece, K / 2 - 16));
+      if (SG == 1 || s0 + SG <= a.groups) sn[j].load(cols.s[j] + min(s0, a.groups - 1), cols.z[j] + min(s0, a.groups - 1));
+      else sn[j].load_part(cols.s[j] + min(s0, a.groups - 1), cols.z[j] + min(s0, a.groups - 1), max(a.groups - s0, 1));
+    }
+  };
+  if (np > 0) {
+    load_rows(0);
+    load_weight(0);
+  }
+  for (int pair = 0; pair < np; ++pair) {
+    char* buf = smem + (pair & 1) * 2 * XB;
 #pragma unroll
-      for (int t = 0; t < SG; ++t) {
-        const int at = min(s0 + t, a.groups - 1);
-        st.s[j][t] = sp[j][at];
-        st.z[j][t] = a.zero ? zp[j][at] : 8;
-      }
+    for (int i = 0; i < CH; ++i) {
+      const int at = tid + i * 512, row = at >> 5, c = at & 31;
+      *(lds_u32x4_t*)(buf + (c >> 4) * XB + row * 256 + (((c & 15) ^ (row & 15)) << 4)) =
+          __builtin_bit_cast(u32x4, permute_row(xs[i]));
     }
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+    for (int j = 0; j < NB; ++j) {
+      q[j] = qn[j];
+      s[j] = sn[j];
+    }
+    if (pair + 1 < np) {
+      load_rows(pair + 1);
+      load_weight(pair + 1);
+    }
+    __syncthreads();  // this buffer is written; the other one's readers are done
+    const char* xb = buf + half * XB;
+    constexpr int PER = 4 / SG;
+    f32x4 p[MB][NB], px[MB];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        st.x[i][t] = u32x4{0u, 0u, 0u, 0u};
-        if (16 * i + l16 < r.rows && k0 + 32 * t + 8 * g < K)
-          __builtin_memcpy(&st.x[i][t], xp + 16ll * i * a.lda + k0 + 32 * t, 16);
-      }
-  };
-  Stage<MB, NB, SG> cur, nxt;
-  int c = w;
-  if (c < nc) load(cur, c);
-  for (; c < nc; c += W) {
-    if (c + W < nc) load(nxt, c + W);
-    f32x4 p[MB][NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) transpose4(cur.q[j]);
+    for (int j = 0; j < NB; ++j) to_operand(q[j], (l16 * 4 + g) * 4);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      constexpr int PER = 4 / SG;  // MFMAs of a group
       s16x8 xf[MB];
 #pragma unroll
-      for (int i = 0; i < MB; ++i) xf[i] = permute_row(cur.x[i][t]);
+      for (int i = 0; i < MB; ++i)
+        xf[i] = *(const lds_s16x8*)(xb + (16 * i + l16) * 256 + (((4 * t + g) ^ l16) << 4));
+      if constexpr (DT == kBF16) {
+        const s16x8 ones = __builtin_bit_cast(s16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if (t % PER == 0) px[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+          px[i] = mfma16x16x32<DT>(xf[i], ones, px[i]);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const float off = 16.0f + (float)cur.z[j][t / PER];
-        const unsigned minus = pack2<DT>(-off, -off);
-        const s16x8 wf = widen<DT>(cur.q[j][t], minus);
+        const unsigned z = s[j].zero(t / PER);
+        const s16x8 wf = widen<DT, true>(q[j][t], bits, minus_of<DT>(z));
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           if (t % PER == 0) p[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
           p[i][j] = mfma16x16x32<DT>(xf[i], wf, p[i][j]);
-          if constexpr (DT == kBF16)
-            p[i][j] = mfma16x16x32<DT>(xf[i], __builtin_bit_cast(s16x8, u32x4{minus, minus, minus, minus}), p[i][j]);
-          if (t % PER == PER - 1) {
-            const float s = to_f32<DT>(cur.s[j][t / PER]);
+        }
+        if (t % PER == PER - 1) {
+          const float sc = s[j].scale(t / PER), off = -16.0f - (float)z;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, p[i][j][v], acc[i][j][v]);
-          }
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const float d = DT == kBF16 ? fmaf(off, px[i][v], p[i][j][v]) : p[i][j][v];
+              acc[i][j][v] = fmaf(sc, d, acc[i][j][v]);
+            }
         }
       }
     }
-    cur = nxt;
   }
 
-  // the waves' sums, in wave order
-#pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) red[w][((i * NB + j) * 4 + v) * 64 + lane] = acc[i][j][v];
+  // odd chunks' sums to the even chunks' waves
   __syncthreads();
+  float* red = (float*)smem + wc * (MB * NB * 256) + lane;
+  if (half == 1) {
 #pragma unroll
-  for (int at = tid; at < MB * NB * 256; at += 64 * W) {
-    float s = red[0][at];
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int v = 1; v < W; ++v) s += red[v][at];
-    const int ln = at & 63, v = (at >> 6) & 3, ij = at >> 8;
-    const int m = ij / NB * 16 + 4 * (ln >> 4) + v, n = n0 + ij % NB * 16 + (ln & 15);
-    if (m < r.rows && n < a.N)
-      ((unsigned short*)a.C)[((long long)r.row0 + m) * a.ldc + n] = (unsigned short)pack2<DT>(s, 0.f);
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) red[((i * NB + j) * 4 + v) * 64] = acc[i][j][v];
+  }
+  __syncthreads();
+  if (half == 0) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int m = 16 * i + 4 * g + v, n = n0 + 16 * j + l16;
+          if (m < r.rows && n < a.N)
+            ((unsigned short*)a.C)[((long long)r.row0 + m) * a.ldc + n] =
+                (unsigned short)pack2<DT>(acc[i][j][v] + red[((i * NB + j) * 4 + v) * 64], 0.f);
+        }
   }
 }
 
-template <int DT, int MB, int NB, int SG>
-hipError_t launch(Args a, hipStream_t s) {
-  constexpr int W = 8;
+// Row tiles x column tiles of a launch, as its kernel numbers them.
+inline long long blocks_of(const Args& a, int bm, int bn) {
+  const long long rows = a.ends ? row_tiles_bound(a.T, a.E, bm, a.zero_tail) : (a.T + bm - 1) / bm;
+  return rows * ((a.N + bn - 1) / bn);
+}
+
+template <int DT, int NB, int SG, int RX, bool ZERO, int W>
+hipError_t launch_few(Args a, hipStream_t s) {
   a.tiles_n = (a.N + 16 * NB - 1) / (16 * NB);
-  const long long rows = a.ends ? row_tiles_bound(a.T, a.E, 16 * MB, a.zero_tail) : (a.T + 16 * MB - 1) / (16 * MB);
-  const long long blocks = rows * a.tiles_n;
+  const long long blocks = blocks_of(a, 16, 16 * NB);
   if (blocks > (1ll << 30)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((gemm_int4<DT, MB, NB, SG, W>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(64 * W), 0, s, a);
+  hipLaunchKernelGGL((gemm_int4_few<DT, NB, SG, RX, ZERO, W, 2>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(64 * W),
+                     0, s, a);
   return hipGetLastError();
 }
 
-template <int DT, int SG>
+template <int DT, int MB, int NB, int SG, bool ZERO>
+hipError_t launch_rows(Args a, hipStream_t s) {
+  a.tiles_n = (a.N + 64 * NB - 1) / (64 * NB);
+  const long long blocks = blocks_of(a, 16 * MB, 64 * NB);
+  if (blocks > (1ll << 30)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((gemm_int4_rows<DT, MB, NB, SG, ZERO>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(512), 0, s,
+                     a);
+  return hipGetLastError();
+}
+
+template <int DT, int SG, int RX, bool ZERO>
+hipError_t pick_few(const Args& a, hipStream_t s) {
+  // Waves a tile: enough to fill the CUs where there are few tiles (1 x 4096 x 4096: 8
+  // waves 4.5 us, 4 5.2), no more where there are many — the chip starts about 3.5
+  // waves a ns (16 x 4096 x 11007: 4 waves 11.7 us, 2 15.0; 64 experts 2048 x 2048 of
+  // 64 rows, 32 columns a tile: 2 waves 27 us, 4 29, 8 43; 16 columns and 2 waves 30).
+  const long long tiles = (long long)(a.ends ? (a.T < a.E ? a.T : a.E) : 1) * ((a.N + 15) / 16);
+  if (tiles >= 4096) return launch_few<DT, 2, SG, RX, ZERO, 2>(a, s);
+  if (tiles > 512) return launch_few<DT, 1, SG, RX, ZERO, 4>(a, s);
+  return launch_few<DT, 1, SG, RX, ZERO, 8>(a, s);
+}
+
+template <int DT, int SG, bool ZERO>
 hipError_t pick(const Args& a, hipStream_t s) {
   const int avg = (a.T + a.E - 1) / a.E;
-  if (avg <= 16) return launch<DT, 1, 1, SG>(a, s);
-  if (avg <= 32) return launch<DT, 2, 2, SG>(a, s);
-  return launch<DT, 4, 2, SG>(a, s);
+  if (a.T <= 4) return pick_few<DT, SG, 1, ZERO>(a, s);
+  if (avg <= 16) return pick_few<DT, SG, 4, ZERO>(a, s);
+  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO>(a, s);
+  if (blocks_of(a, 64, 128) >= 512) return launch_rows<DT, 4, 2, SG, ZERO>(a, s);
+  return launch_rows<DT, 4, 1, SG, ZERO>(a, s);
+}
+
+template <int DT, bool ZERO>
+hipError_t pick_groups(const Args& a, int G, hipStream_t s) {
+  return G == 32 ? pick<DT, 4, ZERO>(a, s) : G == 64 ? pick<DT, 2, ZERO>(a, s) : pick<DT, 1, ZERO>(a, s);
 }
 
 template <int DT>
-hipError_t pick_groups(const Args& a, int G, hipStream_t s) {
-  return G == 32 ? pick<DT, 4>(a, s) : G == 64 ? pick<DT, 2>(a, s) : pick<DT, 1>(a, s);
+hipError_t pick_zero(const Args& a, int G, hipStream_t s) {
+  return a.zero ? pick_groups<DT, true>(a, G, s) : pick_groups<DT, false>(a, G, s);
 }
 
 }  // namespace kint4
@@ -224,6 +641,8 @@ hipError_t int4_gemm(const Int4Problem& p, hipStream_t stream) {
   if (p.N == 0 || p.T == 0 || p.E == 0) return hipSuccess;
   // a chunk's scales are whole groups: G divides 128 or is a multiple of it
   if (p.G < 32 || p.G % 32 || (p.G != 32 && p.G != 64 && p.G % 128) || p.K % p.G) return hipErrorInvalidValue;
+  // row loads are 16 B, at offsets below 2^31 in a tile
+  if ((uintptr_t)p.X % 16 || p.ldx % 8 || p.ldx > (1ll << 23) || p.K > (1 << 23)) return hipErrorInvalidValue;
   kint4::Args a{};
   a.A = p.X;
   a.B = p.q;
@@ -240,9 +659,9 @@ hipError_t int4_gemm(const Int4Problem& p, hipStream_t stream) {
   a.scale = p.scale;
   a.zero = (const unsigned char*)p.zero;
   a.groups = p.K / p.G;
-  a.chunk_g = p.G >= 128 ? p.G / 128 : 1;
-  if (p.dtype == kBF16) return kint4::pick_groups<kBF16>(a, p.G, stream);
-  if (p.dtype == kF16) return kint4::pick_groups<kF16>(a, p.G, stream);
+  a.chunk_g = p.G > 128 ? (unsigned)(((1ll << 32) + p.G / 128 - 1) / (p.G / 128)) : 0u;
+  if (p.dtype == kBF16) return kint4::pick_zero<kBF16>(a, p.G, stream);
+  if (p.dtype == kF16) return kint4::pick_zero<kF16>(a, p.G, stream);
   return hipErrorInvalidValue;
 }
 

@@ -3,7 +3,8 @@ once, ``int4_matmul`` multiplies by it (one weight, or one for each expert).
 
 A weight [K, N] is held by column, as fp8's B operand is: ``q`` [N, K/2] uint8, two
 values a byte, the even k in the low half; ``scale`` [N, K/G] in the rows' dtype
-and ``zero`` [N, K/G] uint8 (None: 8 everywhere) for each group of G values of k:
+and ``zero`` [N, K/G] uint8 (0..15, higher bits are ignored; None: 8 everywhere) for
+each group of G values of k:
 ``W[k, n] = scale[n, k // G] * (q[n, k] - zero[n, k // G])``. G is 32, 64 or a
 multiple of 128, and divides K. Expert weights have a leading dimension [E, ...].
 
@@ -85,7 +86,7 @@ def int4_dequantize(q: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.T
     """The weight that ``(q, scale, zero)`` stand for, float32, [K, N] or [E, K, N] (column-major)."""
     K = _check_weight(q, scale, zero, "int4_dequantize")
     v = torch.stack((q & 15, q >> 4), dim=-1).flatten(-2).float().unflatten(-1, (scale.shape[-1], -1))
-    v = v - (8.0 if zero is None else zero.float().unsqueeze(-1))
+    v = v - (8.0 if zero is None else (zero & 15).float().unsqueeze(-1))
     w = (v * scale.float().unsqueeze(-1)).flatten(-2)
     assert w.shape[-1] == K
     return w.transpose(-1, -2)
@@ -94,6 +95,15 @@ def int4_dequantize(q: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.T
 def _plain(t: torch.Tensor) -> torch.Tensor:
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with 16-byte aligned rows, which the kernels load 16 bytes at a time (K is a
+    multiple of 32, so a copy is aligned)."""
+    x = _prep(x)
+    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
 
 
 def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
@@ -143,6 +153,6 @@ def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
     fresh = out is None
     if fresh:
         out = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    C.int4_matmul(_prep(x), _plain(q), _plain(scale), None if zero is None else _plain(zero),
+    C.int4_matmul(_rows(x), _plain(q), _plain(scale), None if zero is None else _plain(zero),
                   None if ends is None else ends.contiguous(), out, fresh)
     return out
