@@ -317,46 +317,65 @@ void destroy_stream(int64_t stream) {
   check_hip(hipStreamDestroy((hipStream_t)(uintptr_t)stream), "hipStreamDestroy");
 }
 
-// Shared checks of the expert-grouped entry points: `ends` is one running end a
-// group, on the rows' device.
-void check_ends(const at::Tensor& ends, const at::Tensor& x, int64_t E) {
-  TORCH_CHECK(ends.device() == x.device(), "pdmb: ends must be on ", x.device());
-  TORCH_CHECK(ends.scalar_type() == at::kInt || ends.scalar_type() == at::kLong, "pdmb: ends must be int32 or int64");
-  TORCH_CHECK(ends.dim() == 1 && ends.size(0) == E && ends.is_contiguous(), "pdmb: ends must be [", E, "] and contiguous");
+// ---- expert-grouped and 4-bit products -------------------------------------
+// Each entry point returns nothing (and does nothing) when an argument is not
+// as its kernel takes it; ops/grouped.py and ops/int4.py then say what is wrong, or
+// copy what can be used that way and call again. (All tests of a call that fits are
+// made here: they cost the short products less than in Python.)
+
+bool one_device(const at::Tensor& x, const at::Tensor& t) { return t.is_cuda() && t.device() == x.device(); }
+
+bool ends_ok(const at::Tensor& ends, const at::Tensor& x, int64_t E) {
+  return one_device(x, ends) && (ends.scalar_type() == at::kInt || ends.scalar_type() == at::kLong) &&
+         ends.dim() == 1 && ends.size(0) == E && ends.is_contiguous();
 }
 
-void check_fits(std::initializer_list<int64_t> sizes) {
-  for (int64_t v : sizes) TORCH_CHECK(v <= INT32_MAX, "pdmb: size ", v, " exceeds 2^31 - 1");
-}
-
-// Row stride of a matrix whose rows are contiguous and do not overlap.
-int64_t row_stride(const at::Tensor& t, const char* what) {
+// Matrix (of a batch) with contiguous rows that do not overlap; ld: its row stride.
+bool rows_ok(const at::Tensor& t, int64_t* ld) {
   const int64_t rows = t.size(-2), cols = t.size(-1);
-  TORCH_CHECK(cols <= 1 || t.stride(-1) == 1, "pdmb: ", what, " needs contiguous rows");
-  if (rows <= 1) return std::max<int64_t>(cols, 1);
-  TORCH_CHECK(t.stride(-2) >= cols, "pdmb: ", what, " has overlapping rows");
-  return t.stride(-2);
+  *ld = rows <= 1 ? std::max<int64_t>(cols, 1) : t.stride(-2);
+  return (cols <= 1 || t.stride(-1) == 1) && *ld >= cols;
 }
+
+bool fits(std::initializer_list<int64_t> sizes) {
+  for (int64_t v : sizes)
+    if (v > INT32_MAX) return false;
+  return true;
+}
+
+bool records(const at::Tensor& a, const at::Tensor& b) {
+  return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+}
+
+// out as given, or a new one; false if it cannot be written as C.
+bool output(c10::optional<at::Tensor>& out, at::IntArrayRef shape, const at::Tensor& like) {
+  if (!out.has_value()) {
+    out = at::empty(shape, like.options().requires_grad(false));
+    return true;
+  }
+  return one_device(like, *out) && out->scalar_type() == like.scalar_type() && out->sizes() == shape &&
+         !(at::GradMode::is_enabled() && out->requires_grad());
+}
+
+using MaybeTensor = c10::optional<at::Tensor>;
 
 // out[r] = x[r] @ w[e] for the rows r of expert e; w row- or column-major.
-void grouped_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ends, const at::Tensor& out,
-                  bool zero_tail) {
-  TORCH_CHECK(x.is_cuda() && w.device() == x.device() && out.device() == x.device(), "pdmb: tensors must be on one GPU");
-  TORCH_CHECK(x.scalar_type() == w.scalar_type() && x.scalar_type() == out.scalar_type(), "pdmb: dtype mismatch");
-  TORCH_CHECK(x.dim() == 2 && w.dim() == 3 && out.dim() == 2, "pdmb: x [T,K], w [E,K,N], out [T,N] expected");
-  const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(2);
-  TORCH_CHECK(w.size(1) == K && out.size(0) == T && out.size(1) == N, "pdmb: shape mismatch: x ", x.sizes(), ", w ",
-              w.sizes(), ", out ", out.sizes());
-  check_ends(ends, x, E);
-  check_fits({T, K, N, E});
-  const bool colmajor = !(N <= 1 || w.stride(2) == 1);
+MaybeTensor grouped_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ends, MaybeTensor out) {
   pdmb::GroupedProblem p{};
+  if (!x.is_cuda() || !one_device(x, w) || x.dim() != 2 || w.dim() != 3 || x.scalar_type() != w.scalar_type() ||
+      !(x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16))
+    return {};
+  const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(2);
+  if (E < 1 || w.size(1) != K || !ends_ok(ends, x, E) || !fits({T, K, N, E}) || records(x, w)) return {};
+  const bool colmajor = !(N <= 1 || w.stride(2) == 1);
+  if (!rows_ok(x, (int64_t*)&p.lda) || !rows_ok(colmajor ? w.transpose(1, 2) : w, (int64_t*)&p.ldb)) return {};
+  p.zero_tail = !out.has_value();
+  if (!output(out, {T, N}, x) || !rows_ok(*out, (int64_t*)&p.ldc)) return {};
   p.kind = pdmb::kGroupRows;
   p.dtype = dtype_code(x.scalar_type());
-  TORCH_CHECK(p.dtype <= 2, "pdmb: float32 / float16 / bfloat16 only");
   p.A = x.data_ptr();
   p.B = w.data_ptr();
-  p.C = out.data_ptr();
+  p.C = out->data_ptr();
   p.ends = ends.data_ptr();
   p.ends64 = ends.scalar_type() == at::kLong;
   p.E = (int)E;
@@ -364,78 +383,73 @@ void grouped_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& en
   p.M = (int)T;
   p.N = (int)N;
   p.K = (int)K;
-  p.lda = row_stride(x, "x");
-  p.ldb = colmajor ? row_stride(w.transpose(1, 2), "w") : row_stride(w, "w");
-  p.ldc = row_stride(out, "out");
   p.sB = w.stride(0);
   p.b_colmajor = colmajor;
-  p.zero_tail = zero_tail;
   c10::hip::HIPGuard guard(x.device().index());
   check_hip(pdmb::grouped_gemm(p, c10::hip::getCurrentHIPStream(x.device().index()).stream()), "grouped_rows launch");
+  return out;
 }
 
 // out[e] = x_e^T @ dy_e over the rows of expert e.
-void grouped_reduce(const at::Tensor& x, const at::Tensor& dy, const at::Tensor& ends, const at::Tensor& out) {
-  TORCH_CHECK(x.is_cuda() && dy.device() == x.device() && out.device() == x.device(), "pdmb: tensors must be on one GPU");
-  TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.scalar_type() == out.scalar_type(), "pdmb: dtype mismatch");
-  TORCH_CHECK(x.dim() == 2 && dy.dim() == 2 && out.dim() == 3, "pdmb: x [T,M], dy [T,N], out [E,M,N] expected");
-  const int64_t T = x.size(0), M = x.size(1), N = dy.size(1), E = out.size(0);
-  TORCH_CHECK(dy.size(0) == T && out.size(1) == M && out.size(2) == N, "pdmb: shape mismatch: x ", x.sizes(), ", dy ",
-              dy.sizes(), ", out ", out.sizes());
-  check_ends(ends, x, E);
-  check_fits({T, M, N, E});
+MaybeTensor grouped_reduce(const at::Tensor& x, const at::Tensor& dy, const at::Tensor& ends, MaybeTensor out) {
   pdmb::GroupedProblem p{};
+  if (!x.is_cuda() || !one_device(x, dy) || x.dim() != 2 || dy.dim() != 2 || x.scalar_type() != dy.scalar_type() ||
+      !(x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16))
+    return {};
+  const int64_t T = x.size(0), M = x.size(1), N = dy.size(1), E = ends.dim() == 1 ? ends.size(0) : 0;
+  if (E < 1 || dy.size(0) != T || !ends_ok(ends, x, E) || !fits({T, M, N, E}) || records(x, dy)) return {};
+  if (!rows_ok(x, (int64_t*)&p.lda) || !rows_ok(dy, (int64_t*)&p.ldb)) return {};
+  if (!output(out, {E, M, N}, x) || !rows_ok(*out, (int64_t*)&p.ldc)) return {};
+  p.sC = out->stride(0);
+  if (E > 1 && p.sC < M * p.ldc) return {};
   p.kind = pdmb::kGroupReduce;
   p.dtype = dtype_code(x.scalar_type());
-  TORCH_CHECK(p.dtype <= 2, "pdmb: float32 / float16 / bfloat16 only");
   p.A = x.data_ptr();
   p.B = dy.data_ptr();
-  p.C = out.data_ptr();
+  p.C = out->data_ptr();
   p.ends = ends.data_ptr();
   p.ends64 = ends.scalar_type() == at::kLong;
   p.E = (int)E;
   p.T = (int)T;
   p.M = (int)M;
   p.N = (int)N;
-  p.lda = row_stride(x, "x");
-  p.ldb = row_stride(dy, "dy");
-  p.ldc = row_stride(out, "out");
-  p.sC = out.stride(0);
-  TORCH_CHECK(E <= 1 || p.sC >= M * p.ldc, "pdmb: out has overlapping experts");
   c10::hip::HIPGuard guard(x.device().index());
   check_hip(pdmb::grouped_gemm(p, c10::hip::getCurrentHIPStream(x.device().index()).stream()), "grouped_reduce launch");
+  return out;
 }
 
 // out = x @ W^T with W from 4-bit values, scales and zero points (api.h Int4Problem).
-void int4_matmul(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, c10::optional<at::Tensor> zero,
-                 c10::optional<at::Tensor> ends, const at::Tensor& out, bool zero_tail) {
-  TORCH_CHECK(x.is_cuda() && q.device() == x.device() && scale.device() == x.device() && out.device() == x.device() &&
-                  (!zero.has_value() || zero->device() == x.device()),
-              "pdmb: tensors must be on one GPU");
-  TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "pdmb: int4 rows are float16 or bfloat16");
-  TORCH_CHECK(scale.scalar_type() == x.scalar_type() && out.scalar_type() == x.scalar_type(), "pdmb: dtype mismatch");
-  TORCH_CHECK(q.scalar_type() == at::kByte && (!zero.has_value() || zero->scalar_type() == at::kByte),
-              "pdmb: q and zero are uint8");
-  const int64_t lead = ends.has_value() ? 3 : 2;
-  TORCH_CHECK(x.dim() == 2 && out.dim() == 2 && q.dim() == lead && scale.dim() == lead, "pdmb: bad rank");
-  const int64_t T = x.size(0), K = x.size(1), E = lead == 3 ? q.size(0) : 1, N = q.size(-2), J = scale.size(-1);
-  TORCH_CHECK(q.size(-1) * 2 == K && scale.size(-2) == N && (lead == 2 || scale.size(0) == E) && out.size(0) == T &&
-                  out.size(1) == N && J > 0 && K % J == 0,
-              "pdmb: shape mismatch: x ", x.sizes(), ", q ", q.sizes(), ", scale ", scale.sizes(), ", out ", out.sizes());
-  TORCH_CHECK(!zero.has_value() || zero->sizes() == scale.sizes(), "pdmb: zero must have scale's shape");
-  TORCH_CHECK(q.is_contiguous() && scale.is_contiguous() && (!zero.has_value() || zero->is_contiguous()) &&
-                  (uintptr_t)q.data_ptr() % 16 == 0,
-              "pdmb: q, scale and zero must be contiguous, q 16-byte aligned");
-  check_fits({T, K, N, E});
+MaybeTensor int4_matmul(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, MaybeTensor zero,
+                        MaybeTensor ends, MaybeTensor out) {
   pdmb::Int4Problem p{};
+  const int64_t lead = ends.has_value() ? 3 : 2;
+  if (!x.is_cuda() || !one_device(x, q) || !one_device(x, scale) ||
+      !(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16) || scale.scalar_type() != x.scalar_type() ||
+      q.scalar_type() != at::kByte || x.dim() != 2 || q.dim() != lead || scale.dim() != lead)
+    return {};
+  const int64_t T = x.size(0), K = x.size(1), E = lead == 3 ? q.size(0) : 1, N = q.size(-2), J = scale.size(-1);
+  if (E < 1 || q.size(-1) * 2 != K || scale.size(-2) != N || (lead == 3 && scale.size(0) != E) || J < 1 || K % J ||
+      K < 1 || !fits({T, K, N, E}) || records(x, scale))
+    return {};
+  p.G = (int)(K / J);
+  if (p.G % 32 || !(p.G == 32 || p.G == 64 || p.G % 128 == 0)) return {};
+  if (zero.has_value() && (!one_device(x, *zero) || zero->scalar_type() != at::kByte || zero->sizes() != scale.sizes() ||
+                           !zero->is_contiguous()))
+    return {};
+  if (ends.has_value() && !ends_ok(*ends, x, E)) return {};
+  // q is read 16 bytes at a time, the rows 16 bytes at offsets below 2^31 of a tile
+  if (!q.is_contiguous() || !scale.is_contiguous() || (uintptr_t)q.data_ptr() % 16 || !rows_ok(x, (int64_t*)&p.ldx) ||
+      (uintptr_t)x.data_ptr() % 16 || p.ldx % 8 || p.ldx > (1 << 23))
+    return {};
+  p.zero_tail = !out.has_value();
+  if (!output(out, {T, N}, x) || !rows_ok(*out, (int64_t*)&p.ldc)) return {};
   p.dtype = dtype_code(x.scalar_type());
   p.X = x.data_ptr();
   p.q = q.data_ptr();
   p.scale = scale.data_ptr();
   p.zero = zero.has_value() ? zero->data_ptr() : nullptr;
-  p.C = out.data_ptr();
+  p.C = out->data_ptr();
   if (ends.has_value()) {
-    check_ends(*ends, x, E);
     p.ends = ends->data_ptr();
     p.ends64 = ends->scalar_type() == at::kLong;
   }
@@ -443,14 +457,9 @@ void int4_matmul(const at::Tensor& x, const at::Tensor& q, const at::Tensor& sca
   p.T = (int)T;
   p.N = (int)N;
   p.K = (int)K;
-  p.G = (int)(K / J);
-  TORCH_CHECK(p.G % 32 == 0 && (p.G <= 64 || p.G % 128 == 0), "pdmb: group of ", p.G,
-              " (32, 64 or a multiple of 128 only)");
-  p.ldx = row_stride(x, "x");
-  p.ldc = row_stride(out, "out");
-  p.zero_tail = zero_tail;
   c10::hip::HIPGuard guard(x.device().index());
   check_hip(pdmb::int4_gemm(p, c10::hip::getCurrentHIPStream(x.device().index()).stream()), "int4_matmul launch");
+  return out;
 }
 
 std::string kernel_name(int64_t k) { return pdmb::kernel_name((int)k); }
@@ -761,12 +770,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bench", &bench, "native hipEvent timing loop; returns total ms", py::arg("A"),
         py::arg("B"), py::arg("out"), py::arg("iters"), py::arg("warmup"),
         py::arg("graph") = false, py::arg("kernel") = 0, py::arg("splitk") = 0);
-  m.def("grouped_rows", &grouped_rows, "out[r] = x[r] @ w[e] for the rows of expert e", py::arg("x"), py::arg("w"),
-        py::arg("ends"), py::arg("out"), py::arg("zero_tail"));
-  m.def("grouped_reduce", &grouped_reduce, "out[e] = x_e^T @ dy_e", py::arg("x"), py::arg("dy"), py::arg("ends"),
-        py::arg("out"));
-  m.def("int4_matmul", &int4_matmul, "out = x @ W^T, 4-bit W", py::arg("x"), py::arg("q"), py::arg("scale"),
-        py::arg("zero"), py::arg("ends"), py::arg("out"), py::arg("zero_tail"));
+  m.def("grouped_rows", &grouped_rows, "out[r] = x[r] @ w[e] for the rows of expert e (None: not as the kernel takes it)",
+        py::arg("x"), py::arg("w"), py::arg("ends"), py::arg("out"));
+  m.def("grouped_reduce", &grouped_reduce, "out[e] = x_e^T @ dy_e (None: not as the kernel takes it)", py::arg("x"),
+        py::arg("dy"), py::arg("ends"), py::arg("out"));
+  m.def("int4_matmul", &int4_matmul, "out = x @ W^T, 4-bit W (None: not as the kernel takes it)", py::arg("x"),
+        py::arg("q"), py::arg("scale"), py::arg("zero"), py::arg("ends"), py::arg("out"));
   m.def("kernel_name", &kernel_name);
   m.def("plan_shape", &plan_shape, py::arg("dtype"), py::arg("M"), py::arg("N"), py::arg("K"),
         py::arg("batch") = 1, py::arg("kernel") = 0, py::arg("cus") = 0);

@@ -24,6 +24,23 @@ from . import _native
 from .gemm import SUPPORTED_DTYPES, _prep
 
 
+def _native_call(name: str, x, *args):
+    """The kernel's result, or None where an argument is not as the kernel takes it (the
+    caller then finds out why)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        return None
+    try:
+        return getattr(_native.load(), name)(x, *args)
+    except TypeError:  # an argument that is no tensor
+        return None
+
+
+def _must(out: Optional[torch.Tensor], op: str) -> torch.Tensor:
+    if out is None:
+        raise ValueError(f"{op}: out must have contiguous rows that do not overlap, and sizes below 2^31")
+    return out
+
+
 def _check_ends(ends: torch.Tensor, x: torch.Tensor, experts: int, op: str) -> None:
     if not isinstance(ends, torch.Tensor) or ends.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{op}: ends must be an int32 or int64 tensor")
@@ -79,6 +96,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor,
     view of [E, N, K] weights is read in place). Rows behind the last expert's
     are zero in a fresh result and left as they were in ``out``."""
     op = "grouped_matmul"
+    res = _native_call("grouped_rows", x, w, ends, out)
+    if res is not None:
+        return res
     if x.dim() != 2 or w.dim() != 3:
         raise ValueError(f"{op}: x must be 2-D and w 3-D")
     if x.shape[1] != w.shape[1]:
@@ -101,12 +121,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor,
             if hi > lo:
                 res[lo:hi] = torch.matmul(x[lo:hi], w[e])
         return res
-    C = _native.load()
-    fresh = out is None
-    if fresh:
-        out = torch.empty(T, N, dtype=x.dtype, device=x.device)
-    C.grouped_rows(_prep(x), _prep_weight(w), ends.contiguous(), out, fresh)
-    return out
+    return _must(_native_call("grouped_rows", _prep(x), _prep_weight(w), ends.contiguous(), out), op)
 
 
 def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: torch.Tensor,
@@ -116,6 +131,9 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: torch.Tensor,
     [E]; returns [E, K, N], zeros for an expert without rows. The sums are fp32
     and rounded once."""
     op = "grouped_weight_grad"
+    res = _native_call("grouped_reduce", x, dy, ends, out)
+    if res is not None:
+        return res
     if x.dim() != 2 or dy.dim() != 2:
         raise ValueError(f"{op}: x and dy must be 2-D")
     if x.shape[0] != dy.shape[0]:
@@ -137,8 +155,4 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: torch.Tensor,
         for e, lo, hi in _ranges(ends, x.shape[0]):
             res[e] = torch.matmul(x[lo:hi].t(), dy[lo:hi])
         return res
-    C = _native.load()
-    if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    C.grouped_reduce(_prep(x), _prep(dy), ends.contiguous(), out)
-    return out
+    return _must(_native_call("grouped_reduce", _prep(x), _prep(dy), ends.contiguous(), out), op)

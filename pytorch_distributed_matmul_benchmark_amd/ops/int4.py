@@ -18,9 +18,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _native
 from .gemm import _prep
-from .grouped import _check_ends, _check_out, _no_grad, _ranges
+from .grouped import _check_ends, _check_out, _must, _native_call, _no_grad, _ranges
 
 INT4_DTYPES = (torch.float16, torch.bfloat16)
 
@@ -117,6 +116,9 @@ def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
     result and left as they were in ``out``. The weight is frozen: no gradients
     are recorded. In bfloat16 a row with an infinity gives NaN."""
     op = "int4_matmul"
+    res = _native_call("int4_matmul", x, q, scale, zero, ends, out)
+    if res is not None:
+        return res
     if x.dim() != 2:
         raise ValueError(f"{op}: x must be 2-D")
     if x.dtype not in INT4_DTYPES:
@@ -149,10 +151,6 @@ def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
                 if hi > lo:
                     res[lo:hi] = torch.matmul(x[lo:hi].float(), w[e]).to(x.dtype)
         return res
-    C = _native.load()
-    fresh = out is None
-    if fresh:
-        out = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    C.int4_matmul(_rows(x), _plain(q), _plain(scale), None if zero is None else _plain(zero),
-                  None if ends is None else ends.contiguous(), out, fresh)
-    return out
+    return _must(_native_call("int4_matmul", _rows(x), _plain(q), _plain(scale),
+                              None if zero is None else _plain(zero),
+                              None if ends is None else ends.contiguous(), out), op)
