@@ -31,12 +31,18 @@ __device__ __forceinline__ int group_end(const void* ends, int ends64, int T, in
   return (int)(v < 0 ? 0 : v > T ? T : v);
 }
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over 64 lanes
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    v += lane >= d ? o : 0;
-  }
+// v of the lane CTRL names, 0 where there is none (or ROWS leaves the lane out).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int from_lane(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive sum over 64 lanes
+  v += from_lane<0x111>(v);       // 1, 2, 4, 8 lanes back inside a row of 16
+  v += from_lane<0x112>(v);
+  v += from_lane<0x114>(v);
+  v += from_lane<0x118>(v);
+  v += from_lane<0x142, 0xa>(v);  // lane 15 of a row to the next row (rows 1, 3)
+  v += from_lane<0x143, 0xc>(v);  // lane 31 to rows 2, 3
   return v;
 }
 
@@ -45,18 +51,23 @@ struct RowTile {
   int e, row0, rows;  // first row, rows of it in this tile (1 .. BM)
 };
 
-// Tiles of BM rows of groups [c0, c0 + 64), one group a lane: first row and
-// row count of lane's group, and its tile count.
+// Groups [c0, c0 + 64), one a lane: first row, row count and tiles of BM rows, all
+// from one load; `carry` is the end of group c0 - 1 and becomes that of c0 + 63.
+struct LaneGroup {
+  int lo, n, tiles;
+};
 template <int BM>
-__device__ __forceinline__ int lane_tiles(const GroupArgs& a, int e, int& lo, int& n) {
-  lo = 0;
-  n = 0;
-  if (e < a.E || (e == a.E && a.zero_tail)) {
-    lo = group_end(a.ends, a.ends64, a.T, e - 1);
-    const int hi = e < a.E ? group_end(a.ends, a.ends64, a.T, e) : a.T;
-    n = hi > lo ? hi - lo : 0;
-  }
-  return (n + BM - 1) / BM;
+__device__ __forceinline__ LaneGroup lane_group(const GroupArgs& a, int c0, int lane, int& carry) {
+  const int e = c0 + lane;
+  int hi = group_end(a.ends, a.ends64, a.T, min(e, a.E - 1));
+  hi = e < a.E ? hi : a.T;
+  LaneGroup l;
+  const int before = from_lane<0x138>(hi);  // (by every lane: an idle one has nothing to read)
+  l.lo = lane ? before : carry;
+  carry = __builtin_amdgcn_readlane(hi, 63);
+  l.n = e < a.E + (a.zero_tail ? 1 : 0) ? max(hi - l.lo, 0) : 0;
+  l.tiles = (l.n + BM - 1) / BM;
+  return l;
 }
 
 // The group's tile that L of the launch's row-tile x column-tile products
@@ -69,17 +80,12 @@ __device__ __forceinline__ int lane_tiles(const GroupArgs& a, int e, int& lo, in
 // tiles and its L2 serves each operand panel to several of them.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int lane, RowTile& r, int& tn) {
-  int lo, n;
-  int t = lane_tiles<BM>(a, lane, lo, n);
-  int inc = wave_scan(t, lane);
+  int carry = 0;
+  LaneGroup l = lane_group<BM>(a, 0, lane, carry);
+  int inc = wave_scan(l.tiles);
   int total = __builtin_amdgcn_readlane(inc, 63);
-  const int groups = a.E + 1;  // the tail counts as one
-  if (groups > 64) {
-    for (int c0 = 64; c0 < groups; c0 += 64) {
-      int lo2, n2;
-      total += __builtin_amdgcn_readlane(wave_scan(lane_tiles<BM>(a, c0 + lane, lo2, n2), lane), 63);
-    }
-  }
+  for (int c0 = 64; c0 < a.E + 1; c0 += 64)  // (the tail counts as a group)
+    total += __builtin_amdgcn_readlane(wave_scan(lane_group<BM>(a, c0, lane, carry).tiles), 63);
   // XCD-run order over `total` x tiles_n products
   const unsigned prods = (unsigned)total * (unsigned)a.tiles_n;
   const unsigned per = (prods + 7) / 8, x = b & 7, i = b >> 3;
@@ -96,17 +102,18 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int la
     const int tot = __builtin_amdgcn_readlane(inc, 63);
     if (slot < base + tot) break;
     base += tot;
+    if (c0 == 0) carry = group_end(a.ends, a.ends64, a.T, min(63, a.E - 1));
     c0 += 64;
-    t = lane_tiles<BM>(a, c0 + lane, lo, n);
-    inc = wave_scan(t, lane);
+    l = lane_group<BM>(a, c0, lane, carry);
+    inc = wave_scan(l.tiles);
   }
   const unsigned long long at = __ballot(slot < base + inc);  // first lane whose tiles reach slot
-  const int l = __builtin_ctzll(at);
-  const int before = base + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(t, l);
+  const int k = __builtin_ctzll(at);
+  const int before = base + __builtin_amdgcn_readlane(inc, k) - __builtin_amdgcn_readlane(l.tiles, k);
   const int off = (slot - before) * BM;
-  r.e = c0 + l;
-  r.row0 = __builtin_amdgcn_readlane(lo, l) + off;
-  r.rows = min(BM, __builtin_amdgcn_readlane(n, l) - off);
+  r.e = c0 + k;
+  r.row0 = __builtin_amdgcn_readlane(l.lo, k) + off;
+  r.rows = min(BM, __builtin_amdgcn_readlane(l.n, k) - off);
   return true;
 }
 

@@ -17,10 +17,13 @@
 // In fp32 MFMA step (h, j) multiplies k = 16 h + 4 g + j: any order of k that
 // both operands share gives the same sum of products.
 //
-// This kernel stages global -> registers -> LDS, so that any alignment and any
-// size is right: chunks past an edge are zero, chunks that an edge cuts are read by
-// the element. Two LDS stages, one barrier a K-tile, the next K-tile's loads in
-// flight during a K-tile's MFMAs.
+// This kernel stages global -> registers -> LDS: PF K-tiles in flight in
+// registers, two LDS stages, one barrier a K-tile. BUF: operands at a multiple
+// of 4 bytes come as 16-byte buffer loads whose descriptor ends with the tile's last
+// row (KC) or k (KS), moved along k, so that what is not there reads as zero with no
+// branch (a branch around a load makes hipcc wait for later loads too); only a row
+// that ends inside 16 bytes is masked, in its last K-tile. Others are read with any
+// alignment, by the element at the edges.
 #include "api.h"
 #include "grouped.h"
 
@@ -32,15 +35,12 @@ constexpr int NT = 256;
 template <int DT>
 constexpr int esize() { return DT == kF32 ? 4 : 2; }
 
-// 16 bytes at p, of which `avail` elements are inside the operand. VEC: p is
-// 16-B aligned and an edge never cuts a chunk.
-template <int DT, bool VEC>
+// 16 bytes at p (any alignment), of which `avail` elements are inside the operand.
+template <int DT>
 __device__ __forceinline__ u32x4 load_chunk(const char* p, int avail) {
   constexpr int ES = esize<DT>(), EPC = 16 / ES;
   u32x4 v = {0u, 0u, 0u, 0u};
-  if constexpr (VEC) {
-    if (avail > 0) v = *(const u32x4*)p;
-  } else if (avail >= EPC) {
+  if (avail >= EPC) {
     __builtin_memcpy(&v, p, 16);
   } else if (avail > 0) {
     if constexpr (ES == 4) {
@@ -56,22 +56,42 @@ __device__ __forceinline__ u32x4 load_chunk(const char* p, int avail) {
   return v;
 }
 
+// The first `avail` elements of a chunk, zeros for the rest.
+template <int DT>
+__device__ __forceinline__ u32x4 keep(u32x4 v, int avail) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == kF32) v[i] = i < avail ? v[i] : 0u;
+    else v[i] = 2 * i + 1 < avail ? v[i] : 2 * i < avail ? v[i] & 0xffffu : 0u;
+  }
+  return v;
+}
+
 // One operand tile of R rows (or columns) x one K-tile.
-template <int DT, bool KC, int R>
+template <int DT, bool KC, int R, bool BUF>
 struct Tile {
   static constexpr int ES = esize<DT>(), EPC = 16 / ES, BK = 128 / ES;
   static constexpr int BYTES = R * 128;
   static constexpr int CH = (R * 8 + NT - 1) / NT;  // chunks a thread
   static constexpr int PITCH = R * ES;              // KS image: bytes of one k
-  static_assert(KC || R >= 128, "KS swizzle spans 8 units");
+  static constexpr int CPK = PITCH / 16;
+  static_assert(KC || R * ES >= 256, "the KS swizzles' units");
 
+  const char* p;   // first row / column, k = 0
+  long long ld;    // leading stride
+  int rows, ks;    // what there is of it
+  int first;       // lane's offset of chunk 0 in bytes (BUF)
+
+  __device__ __forceinline__ Tile(const char* p_, long long ld_, int rows_, int ks_, int tid)
+      : p(p_), ld(ld_), rows(rows_ < R ? rows_ : R), ks(ks_) {
+    first = KC ? (tid >> 3) * (int)(ld * ES) + (tid & 7) * 16 : tid / CPK * (int)(ld * ES) + tid % CPK * 16;
+  }
   // LDS offset of chunk idx
   __device__ static __forceinline__ int at(int idx) {
     if constexpr (KC) {
       const int r = idx >> 3, c = idx & 7;
       return r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
     } else {
-      constexpr int CPK = PITCH / 16;
       const int k = idx / CPK, c = idx % CPK;
       if constexpr (ES == 2) {
         const int s = (k & 3) | (((k >> 3) & 1) << 2);
@@ -81,25 +101,38 @@ struct Tile {
       }
     }
   }
-  // Global loads of K-tile at k0: p is the operand at its first row / column
-  // and k = 0, ld its leading stride, `rows` and `ks` what is left of it.
-  template <bool VEC>
-  __device__ static __forceinline__ void load(u32x4 (&v)[CH], const char* p, long long ld, int rows, int k0, int ks,
-                                              int tid) {
+  // Global loads of the K-tile at k0 (past ks: zeros).
+  __device__ __forceinline__ void load(u32x4 (&v)[CH], int k0, int tid) const {
+    if constexpr (BUF) {
+      // from here to the last element of the tile's last row (KC) or k (KS)
+      const long long from = KC ? (long long)k0 * ES : (long long)k0 * ld * ES;
+      const long long bytes = (KC ? (long long)(rows - 1) * ld + ks : (long long)(ks - 1) * ld + rows) * ES - from;
+      const u32x4 d = make_rsrc(p + from, (bytes + 3) & ~3ll);  // (a dword that the end cuts counts as inside)
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((char*)(p + from), 0, (int)d.z, 0x00020000);
+      const int step = (int)(ld * ES) * (KC ? 32 : NT / CPK);  // bytes between a lane's chunks
+      const int out = KC && (tid & 7) * EPC >= ks - k0 ? (int)0x80000000 : 0;  // k past the end of a row
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int idx = tid + i * NT;
-      if constexpr (KC) {
-        const int r = idx >> 3, k = k0 + (idx & 7) * EPC;
-        v[i] = load_chunk<DT, VEC>(p + ((long long)r * ld + k) * ES, r < rows ? ks - k : 0);
-      } else {
-        constexpr int CPK = PITCH / 16;
-        const int k = k0 + idx / CPK, c = (idx % CPK) * EPC;
-        v[i] = load_chunk<DT, VEC>(p + ((long long)k * ld + c) * ES, k < ks ? rows - c : 0);
+      for (int i = 0; i < CH; ++i)
+        v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (first + i * step) | out, 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int idx = tid + i * NT;
+        if constexpr (KC) {
+          const int r = idx >> 3, k = k0 + (idx & 7) * EPC;
+          v[i] = load_chunk<DT>(p + ((long long)r * ld + k) * ES, r < rows ? ks - k : 0);
+        } else {
+          const int k = k0 + idx / CPK, c = (idx % CPK) * EPC;
+          v[i] = load_chunk<DT>(p + ((long long)k * ld + c) * ES, k < ks ? rows - c : 0);
+        }
       }
     }
   }
-  __device__ static __forceinline__ void store(char* lds, const u32x4 (&v)[CH], int tid) {
+  __device__ __forceinline__ void store(char* lds, u32x4 (&v)[CH], int k0, int tid) const {
+    if (BUF && KC && ks % EPC && k0 + BK > ks) {  // the row ends inside 16 bytes: what follows it is not zero
+#pragma unroll
+      for (int i = 0; i < CH; ++i) v[i] = keep<DT>(v[i], ks - k0 - (tid & 7) * EPC);
+    }
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int idx = tid + i * NT;
@@ -114,15 +147,15 @@ struct Tile {
       return *(const lds_u32x4_t*)(lds + r * 128 + (((4 * h + g) ^ ((r >> 1) & 7)) << 4));
     } else if constexpr (ES == 2) {
       const int q4 = l16 >> 2, p4 = l16 & 3, u = r0 >> 4;
-      const char* p = lds + (32 * h + 8 * g + q4) * PITCH + ((u ^ (q4 | ((g & 1) << 2))) << 5) + p4 * 8;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * PITCH));
+      const char* q = lds + (32 * h + 8 * g + q4) * PITCH + ((u ^ (q4 | ((g & 1) << 2))) << 5) + p4 * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * PITCH));
       return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      const char* p = lds + (16 * h + 4 * g) * PITCH + (((r0 >> 4) ^ g) << 6) + l16 * 4;
+      const char* q = lds + (16 * h + 4 * g) * PITCH + (((r0 >> 4) ^ g) << 6) + l16 * 4;
       u32x4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = *(const __attribute__((address_space(3))) unsigned*)(p + j * PITCH);
+      for (int j = 0; j < 4; ++j) v[j] = *(const __attribute__((address_space(3))) unsigned*)(q + j * PITCH);
       return v;
     }
   }
@@ -140,11 +173,11 @@ __device__ __forceinline__ void mma(f32x4& acc, const u32x4& b, const u32x4& a) 
   }
 }
 
-// Four columns of one row, `left` of them inside C. ALIGNED: 4 elements at once.
-template <int DT, bool ALIGNED>
-__device__ __forceinline__ void store4(char* p, const f32x4& v, int left) {
+// Four columns of one row, `left` of them inside C; whole: 4 elements at once where they all are.
+template <int DT>
+__device__ __forceinline__ void store4(char* p, const f32x4& v, int left, bool whole) {
   if constexpr (DT == kF32) {
-    if (ALIGNED && left >= 4) {
+    if (whole && left >= 4) {
       *(f32x4*)p = v;
     } else {
 #pragma unroll
@@ -153,7 +186,7 @@ __device__ __forceinline__ void store4(char* p, const f32x4& v, int left) {
     }
   } else {
     const u32x2 w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-    if (ALIGNED && left >= 4) {
+    if (whole && left >= 4) {
       *(u32x2*)p = w;
     } else {
 #pragma unroll
@@ -163,16 +196,14 @@ __device__ __forceinline__ void store4(char* p, const f32x4& v, int left) {
   }
 }
 
-// RED: `reduce` (A and B are both KS). BM x 128 tile, 4 waves: 2 x 2 for BM >=
-// 64, else 1 x 4. VEC: 16-B aligned operands whose edges fall between chunks,
-// and a C that takes 4 elements at once.
-template <int DT, bool RED, bool B_KC, int BM, bool VEC>
-__global__ void __launch_bounds__(NT) grouped(GroupArgs a) {
-  constexpr int BN = 128, ES = esize<DT>();
-  using TA = Tile<DT, !RED, BM>;
-  using TB = Tile<DT, B_KC, BN>;
+// RED: `reduce` (A and B are both KS). BM x BN tile, WR x 4 / WR waves.
+template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, bool BUF>
+__global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
+  constexpr int ES = esize<DT>();
+  using TA = Tile<DT, !RED, BM, BUF>;
+  using TB = Tile<DT, B_KC, BN, BUF>;
   constexpr int BK = TA::BK;
-  constexpr int WR = BM >= 64 ? 2 : 1, WC = 4 / WR;
+  constexpr int WC = 4 / WR;
   constexpr int MB = BM / WR / 16, NB = BN / WC / 16;
   constexpr int STAGE = TA::BYTES + TB::BYTES;
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
@@ -184,12 +215,12 @@ __global__ void __launch_bounds__(NT) grouped(GroupArgs a) {
   const char *Ap, *Bp;
   char* Cp;
   int rows, cols, ks;  // of this tile: rows of C left, columns of C left, the sum's length
-  bool zero = false;
   if constexpr (RED) {
     const int per = a.tiles_m * a.tiles_n;
     const int e = blockIdx.x / per, t = blockIdx.x - e * per;
     const int m0 = t / a.tiles_n * BM, n0 = t % a.tiles_n * BN;
-    const int r0 = group_end(a.ends, a.ends64, a.T, e - 1), r1 = group_end(a.ends, a.ends64, a.T, e);
+    const int r0 = __builtin_amdgcn_readfirstlane(group_end(a.ends, a.ends64, a.T, e - 1));
+    const int r1 = __builtin_amdgcn_readfirstlane(group_end(a.ends, a.ends64, a.T, e));
     ks = r1 > r0 ? r1 - r0 : 0;
     rows = a.M - m0;
     cols = a.N - n0;
@@ -200,13 +231,13 @@ __global__ void __launch_bounds__(NT) grouped(GroupArgs a) {
     RowTile r;
     int tn;
     if (!find_tile<BM>(a, blockIdx.x, lane, r, tn)) return;
-    zero = r.e == a.E;
+    const bool zero = r.e == a.E;
     ks = zero ? 0 : a.K;
     rows = r.rows;
     cols = a.N - tn * BN;
     Ap = (const char*)a.A + (long long)r.row0 * a.lda * ES;
     Bp = (const char*)a.B + ((long long)(zero ? 0 : r.e) * a.sB + (long long)tn * BN * (B_KC ? a.ldb : 1)) * ES;
-    Cp = (char*)a.C + ((long long)r.row0 * a.ldc + tn * BN) * ES;
+    Cp = (char*)a.C + ((long long)r.row0 * a.ldc + (long long)tn * BN) * ES;
   }
 
   f32x4 acc[MB][NB];
@@ -216,34 +247,44 @@ __global__ void __launch_bounds__(NT) grouped(GroupArgs a) {
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int nk = (ks + BK - 1) / BK;
-  u32x4 va[TA::CH], vb[TB::CH];
   if (nk > 0) {
-    TA::template load<VEC>(va, Ap, a.lda, rows, 0, ks, tid);
-    TB::template load<VEC>(vb, Bp, a.ldb, cols, 0, ks, tid);
-  }
-  for (int t = 0; t < nk; ++t) {
-    char* st = smem + (t & 1) * STAGE;
-    TA::store(st, va, tid);
-    TB::store(st + TA::BYTES, vb, tid);
-    if (t + 1 < nk) {
-      TA::template load<VEC>(va, Ap, a.lda, rows, (t + 1) * BK, ks, tid);
-      TB::template load<VEC>(vb, Bp, a.ldb, cols, (t + 1) * BK, ks, tid);
+    const TA ta(Ap, a.lda, rows, ks, tid);
+    const TB tb(Bp, a.ldb, cols, ks, tid);
+    u32x4 va[PF][TA::CH], vb[PF][TB::CH];
+#pragma unroll
+    for (int d = 0; d < PF; ++d) {
+      ta.load(va[d], d * BK, tid);
+      tb.load(vb[d], d * BK, tid);
     }
-    __syncthreads();  // this stage is written; the other one's readers are done
+    for (int t0 = 0; t0 < nk; t0 += PF) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 fa[MB], fb[NB];
+      for (int d = 0; d < PF; ++d) {
+        const int t = t0 + d;
+        if (PF > 1 && t >= nk) break;
+        char* st = smem + (t & 1) * STAGE;
+        ta.store(st, va[d], t * BK, tid);
+        tb.store(st + TA::BYTES, vb[d], t * BK, tid);
+        ta.load(va[d], (t + PF) * BK, tid);
+        tb.load(vb[d], (t + PF) * BK, tid);
+        // this stage is written; the other one's readers are done (LDS only: loads stay in flight)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < MB; ++i) fa[i] = TA::frag(st, wr * (BM / WR) + i * 16, h, l16, g);
+        for (int h = 0; h < 2; ++h) {
+          u32x4 fa[MB], fb[NB];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) fb[j] = TB::frag(st + TA::BYTES, wc * (BN / WC) + j * 16, h, l16, g);
+          for (int i = 0; i < MB; ++i) fa[i] = TA::frag(st, wr * (BM / WR) + i * 16, h, l16, g);
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+          for (int j = 0; j < NB; ++j) fb[j] = TB::frag(st + TA::BYTES, wc * (BN / WC) + j * 16, h, l16, g);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) mma<DT>(acc[i][j], fb[j], fa[i]);
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) mma<DT>(acc[i][j], fb[j], fa[i]);
+        }
+      }
     }
   }
 
+  const bool whole = (uintptr_t)a.C % (4 * ES) == 0 && a.ldc % 4 == 0 && a.sC % 4 == 0;
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
     const int r = wr * (BM / WR) + i * 16 + l16;
@@ -251,53 +292,57 @@ __global__ void __launch_bounds__(NT) grouped(GroupArgs a) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const int c = wc * (BN / WC) + j * 16 + 4 * g;
-        store4<DT, VEC>(Cp + ((long long)r * a.ldc + c) * ES, acc[i][j], cols - c);
+        store4<DT>(Cp + ((long long)r * a.ldc + c) * ES, acc[i][j], cols - c, whole);
       }
     }
   }
 }
 
-template <int DT, bool RED, bool B_KC, int BM>
-hipError_t launch(const GroupArgs& a, bool vec, unsigned grid, hipStream_t s) {
-  if (vec)
-    hipLaunchKernelGGL((grouped<DT, RED, B_KC, BM, true>), dim3(grid), dim3(NT), 0, s, a);
+template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF>
+hipError_t launch(GroupArgs a, bool buf, hipStream_t s) {
+  a.tiles_m = (a.M + BM - 1) / BM;
+  a.tiles_n = (a.N + BN - 1) / BN;
+  const long long blocks = RED ? (long long)a.E * a.tiles_m * a.tiles_n
+                               : (row_tiles_bound(a.T, a.E, BM, a.zero_tail) * a.tiles_n + 7) / 8 * 8;
+  if (blocks > (1ll << 30)) return hipErrorInvalidValue;
+  if (buf)
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, PF, true>), dim3((unsigned)blocks), dim3(NT), 0, s, a);
   else
-    hipLaunchKernelGGL((grouped<DT, RED, B_KC, BM, false>), dim3(grid), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, false>), dim3((unsigned)blocks), dim3(NT), 0, s, a);
   return hipGetLastError();
 }
 
 template <int DT, bool B_KC>
-hipError_t launch_rows(GroupArgs a, bool vec, hipStream_t s) {
+hipError_t launch_rows(const GroupArgs& a, bool buf, hipStream_t s) {
   // Rows a group has on average: a tile taller than that computes rows that
   // no group has, one shorter reads the weights once more for each tile.
   const int avg = (a.T + a.E - 1) / a.E;
-  const int bm = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
-  a.tiles_n = (a.N + 127) / 128;
-  const long long prods = row_tiles_bound(a.T, a.E, bm, a.zero_tail) * a.tiles_n;
-  if (prods > (1ll << 30)) return hipErrorInvalidValue;
-  const unsigned grid = (unsigned)((prods + 7) / 8 * 8);
-  switch (bm) {
-    case 16: return launch<DT, false, B_KC, 16>(a, vec, grid, s);
-    case 32: return launch<DT, false, B_KC, 32>(a, vec, grid, s);
-    case 64: return launch<DT, false, B_KC, 64>(a, vec, grid, s);
-    default: return launch<DT, false, B_KC, 128>(a, vec, grid, s);
+  if (avg <= 16) return launch<DT, false, B_KC, 16, 128, 1, 1>(a, buf, s);
+  if constexpr (DT == kF32) {
+    // an MFMA of 4 k takes as long as one of 32 in 16 bits: small tiles lose nothing to
+    // loads, and pad groups and widths less (8 experts of 512 rows, 2048 x 2048: 32 x 64
+    // 306 us, 64 x 64 315, 64 x 128 345, 128 x 128 402; 16 of 85, 1001 x 1416: 53, 60, 75)
+    if (avg <= 256) return launch<DT, false, B_KC, 32, 64, 2, 2>(a, buf, s);
+    return launch<DT, false, B_KC, 64, 64, 2, 2>(a, buf, s);
+  } else {
+    if (avg <= 32) return launch<DT, false, B_KC, 32, 128, 1, 1>(a, buf, s);
+    if (avg <= 64) return launch<DT, false, B_KC, 64, 128, 2, 1>(a, buf, s);
+    return launch<DT, false, B_KC, 128, 128, 2, 1>(a, buf, s);
   }
 }
 
 template <int DT>
-hipError_t launch_reduce(GroupArgs a, bool vec, hipStream_t s) {
-  a.tiles_m = (a.M + 127) / 128;
-  a.tiles_n = (a.N + 127) / 128;
-  const long long blocks = (long long)a.E * a.tiles_m * a.tiles_n;
-  if (blocks > (1ll << 30)) return hipErrorInvalidValue;
-  return launch<DT, true, false, 128>(a, vec, (unsigned)blocks, s);
+hipError_t launch_reduce(const GroupArgs& a, bool buf, hipStream_t s) {
+  if constexpr (DT == kF32) return launch<DT, true, false, 64, 64, 2, 2>(a, buf, s);
+  return launch<DT, true, false, 128, 128, 2, 1>(a, buf, s);
 }
 
 }  // namespace kgrp
 
-static bool vec_ok(const void* p, long long ld, long long batch, int es, int edge) {
-  const int epc = 16 / es;
-  return (uintptr_t)p % 16 == 0 && ld % epc == 0 && batch % epc == 0 && edge % epc == 0;
+// Buffer loads take any multiple of 4 bytes; their offsets stay below 2^31 in 128
+// rows (KC) or 64 k (KS) of an operand.
+static bool buf_ok(const void* p, long long ld, long long batch, int es) {
+  return (uintptr_t)p % 4 == 0 && ld * es % 4 == 0 && batch * es % 4 == 0 && ld * es <= (1ll << 23);
 }
 
 hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
@@ -322,26 +367,24 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
   a.sB = p.sB;
   a.sC = p.sC;
   a.zero_tail = p.zero_tail;
-  const bool c_ok = (uintptr_t)p.C % (4 * es) == 0 && p.ldc % 4 == 0 && p.sC % 4 == 0;
-  const bool vec = c_ok && vec_ok(p.A, p.lda, 0, es, red ? p.M : p.K) &&
-                   vec_ok(p.B, p.ldb, p.sB, es, red || !p.b_colmajor ? p.N : p.K);
+  const bool buf = buf_ok(p.A, p.lda, 0, es) && buf_ok(p.B, p.ldb, p.sB, es);
   const int avg = (p.T + p.E - 1) / p.E;
-  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 192) && (red || p.K > 0) &&
+  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 96) && (red || p.K > 0) &&
       grouped_w4_ok(a, red, p.b_colmajor))
     return grouped_w4(a, p.dtype, red, p.b_colmajor, stream);
   switch (p.dtype) {
     case kF32:
-      return red            ? kgrp::launch_reduce<kF32>(a, vec, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kF32, true>(a, vec, stream)
-                            : kgrp::launch_rows<kF32, false>(a, vec, stream);
+      return red            ? kgrp::launch_reduce<kF32>(a, buf, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kF32, true>(a, buf, stream)
+                            : kgrp::launch_rows<kF32, false>(a, buf, stream);
     case kF16:
-      return red            ? kgrp::launch_reduce<kF16>(a, vec, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kF16, true>(a, vec, stream)
-                            : kgrp::launch_rows<kF16, false>(a, vec, stream);
+      return red            ? kgrp::launch_reduce<kF16>(a, buf, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kF16, true>(a, buf, stream)
+                            : kgrp::launch_rows<kF16, false>(a, buf, stream);
     case kBF16:
-      return red            ? kgrp::launch_reduce<kBF16>(a, vec, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kBF16, true>(a, vec, stream)
-                            : kgrp::launch_rows<kBF16, false>(a, vec, stream);
+      return red            ? kgrp::launch_reduce<kBF16>(a, buf, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kBF16, true>(a, buf, stream)
+                            : kgrp::launch_rows<kBF16, false>(a, buf, stream);
     default:
       return hipErrorInvalidValue;
   }
