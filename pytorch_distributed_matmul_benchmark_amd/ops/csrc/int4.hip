@@ -109,83 +109,104 @@ __device__ __forceinline__ s16x8 widen(unsigned d, const Bits& b, const Minus& m
   return __builtin_bit_cast(s16x8, v);
 }
 
-// G = 32: SG = 4 scales and zero points a chunk of 128 k, 64: 2, 128 and more: 1.
-// Scales and zero points of C neighbouring chunks of one column, as loaded; ZERO:
-// zero points are given (otherwise 8).
-template <int BYTES>
-struct Raw {  // BYTES from any address in as few loads as there are dwords
-  unsigned w[(BYTES + 3) / 4];
-  __device__ __forceinline__ void load(const void* p) {
-    if constexpr (BYTES == 1) w[0] = *(const unsigned char*)p;
-    else if constexpr (BYTES == 2) { unsigned short v; __builtin_memcpy(&v, p, 2); w[0] = v; }
-    else __builtin_memcpy(w, p, BYTES);
-  }
-  __device__ __forceinline__ unsigned half(int i) const { return i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu; }
-  __device__ __forceinline__ unsigned byte(int i) const { return (w[i >> 2] >> (8 * (i & 3))) & 255u; }
-};
-template <int DT, int SG, int C, bool ZERO>
+// A chunk of 128 k has SG scales and zero points of a column: G = 32: 4, 64: 2, 128 and
+// more: 1. ZERO: zero points are given (otherwise 8).
+template <int SG, int DT, bool ZERO>
 struct Scales {
-  static constexpr int N = SG * C;
-  Raw<2 * N> s;
-  Raw<N> z;
-  __device__ __forceinline__ void load(const unsigned short* sp, const unsigned char* zp) {
-    s.load(sp);
-    if constexpr (ZERO) z.load(zp);
-  }
+  unsigned s[(SG + 1) / 2], z;
   __device__ __forceinline__ void load_lds(const char* sp, const char* zp) {
     typedef __attribute__((address_space(3))) unsigned lds_u32;
     typedef __attribute__((address_space(3))) unsigned short lds_u16;
     typedef __attribute__((address_space(3))) unsigned char lds_u8;
-    static_assert(C == 1, "one chunk");
     if constexpr (SG == 1) {
-      s.w[0] = *(const lds_u16*)sp;
-      if constexpr (ZERO) z.w[0] = *(const lds_u8*)zp;
+      s[0] = *(const lds_u16*)sp;
+      if constexpr (ZERO) z = *(const lds_u8*)zp;
     } else if constexpr (SG == 2) {
-      s.w[0] = *(const lds_u32*)sp;
-      if constexpr (ZERO) z.w[0] = *(const lds_u16*)zp;
+      s[0] = *(const lds_u32*)sp;
+      if constexpr (ZERO) z = *(const lds_u16*)zp;
     } else {
       const u32x2 v = *(const lds_u32x2*)sp;
-      s.w[0] = v.x;
-      s.w[1] = v.y;
-      if constexpr (ZERO) z.w[0] = *(const lds_u32*)zp;
-    }
-  }
-  // one by one, the last group repeated: what is left of a column
-  __device__ __forceinline__ void load_part(const unsigned short* sp, const unsigned char* zp, int groups) {
-#pragma unroll
-    for (int t = 0; t < (2 * N + 3) / 4; ++t) s.w[t] = 0;
-#pragma unroll
-    for (int t = 0; t < (N + 3) / 4; ++t) z.w[t] = 0;
-#pragma unroll
-    for (int t = 0; t < N; ++t) {
-      s.w[t >> 1] |= (unsigned)sp[min(t, groups - 1)] << (16 * (t & 1));
-      if constexpr (ZERO) z.w[t >> 2] |= (unsigned)zp[min(t, groups - 1)] << (8 * (t & 3));
+      s[0] = v.x;
+      s[1] = v.y;
+      if constexpr (ZERO) z = *(const lds_u32*)zp;
     }
   }
   __device__ __forceinline__ float scale(int t) const {
-    if constexpr (DT == kBF16) return __uint_as_float(t & 1 ? s.w[t >> 1] & 0xffff0000u : s.w[t >> 1] << 16);
-    else return to_f32<DT>((unsigned short)s.half(t));
+    if constexpr (DT == kBF16) return __uint_as_float(t & 1 ? s[t >> 1] & 0xffff0000u : s[t >> 1] << 16);
+    else return to_f32<DT>((unsigned short)(s[t >> 1] >> (16 * (t & 1))));
   }
-  __device__ __forceinline__ unsigned zero(int t) const { return ZERO ? z.byte(t) & 15u : 8u; }
+  __device__ __forceinline__ unsigned zero(int t) const { return ZERO ? (z >> (8 * t)) & 15u : 8u; }
 };
 
-// A lane's columns. Loads: column 16 j + (lane >> 2), 16-B piece lane & 3. Scales:
-// column 16 j + l16.
-template <int NB>
-struct Columns {
-  const unsigned char* q[NB];
-  const unsigned short* s[NB];
-  const unsigned char* z[NB];
-  __device__ __forceinline__ Columns(const Args& a, int e, int n0, int lane) {
+// Scales and zero points of COLS columns and KB chunks go to LDS before they are
+// used, 8 groups a lane: read where they are used they cost a cache line look-up for
+// every lane (a 16 x 4096 x 11007 product with groups of 32: 128 of a chunk's 208).
+// [column][KB * SG groups], 8 bytes between columns against bank conflicts.
+template <int DT, int COLS, int SG, int KB, bool ZERO, int THREADS>
+struct ScaleBlock {
+  static constexpr int NG = KB * SG, SP = 2 * NG + 8, ZP = NG + 8, BYTES = COLS * (SP + ZP);
+  static constexpr int PIECES = COLS * NG / 8, CH = (PIECES + THREADS - 1) / THREADS;
+  u32x4 s[CH];
+  u32x2 z[CH];
+  // groups from g0 of columns from n0 (of expert e's `first`); what is not there is zero
+  __device__ __forceinline__ void load(const Args& a, long long first, int n0, int g0, int tid) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const long long base = (long long)e * a.N;
-      const long long nq = base + min(n0 + 16 * j + (lane >> 2), a.N - 1);
-      const long long ns = base + min(n0 + 16 * j + (lane & 15), a.N - 1);
-      q[j] = (const unsigned char*)a.B + nq * (a.K / 2) + 16 * (lane & 3);
-      s[j] = (const unsigned short*)a.scale + ns * a.groups;
-      z[j] = a.zero + ns * a.groups;
+    for (int i = 0; i < CH; ++i) {
+      const int at = tid + i * THREADS, col = at / (NG / 8), gr = g0 + at % (NG / 8) * 8;
+      const long long off = (first + min(n0 + col, a.N - 1)) * a.groups + gr;
+      const unsigned short* sp = (const unsigned short*)a.scale + off;
+      const unsigned char* zp = a.zero + off;
+      s[i] = u32x4{0u, 0u, 0u, 0u};
+      z[i] = u32x2{0u, 0u};
+      if (gr + 8 <= a.groups) {
+        __builtin_memcpy(&s[i], sp, 16);
+        if constexpr (ZERO) __builtin_memcpy(&z[i], zp, 8);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 7; ++t)
+          if (gr + t < a.groups) {
+            s[i][t >> 1] |= (unsigned)sp[t] << (16 * (t & 1));
+            if constexpr (ZERO) z[i][t >> 2] |= (unsigned)zp[t] << (8 * (t & 3));
+          }
+      }
     }
+  }
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int at = tid + i * THREADS, col = at / (NG / 8), gr = at % (NG / 8) * 8;
+      if (PIECES % THREADS == 0 || at < PIECES) {
+        char* p = lds + col * SP + 2 * gr;
+        *(lds_u32x2*)p = u32x2{s[i][0], s[i][1]};
+        *(lds_u32x2*)(p + 8) = u32x2{s[i][2], s[i][3]};
+        if constexpr (ZERO) *(lds_u32x2*)(lds + COLS * SP + col * ZP + gr) = z[i];
+      }
+    }
+  }
+  // column c, SG groups from `at` of the block
+  __device__ static __forceinline__ void read(Scales<SG, DT, ZERO>& v, const char* lds, int c, int at) {
+    v.load_lds(lds + c * SP + 2 * at, lds + COLS * SP + c * ZP + at);
+  }
+};
+
+// Where a lane loads of column block j: column 16 j + (lane >> 2), 16-byte piece lane & 3.
+template <int NB>
+struct Weights {
+  const unsigned char* p[NB];
+  int tail;  // moves the piece inside a partial last chunk (any weight will do: the rows are zero there)
+  __device__ __forceinline__ Weights(const Args& a, long long first, int n0, int lane) {
+    const int piece = 16 * (lane & 3), part = a.K % 128;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      p[j] = (const unsigned char*)a.B + (first + min(n0 + 16 * j + (lane >> 2), a.N - 1)) * (a.K / 2) + piece;
+    tail = part ? min(piece, part / 2 - 16) - piece : 0;
+  }
+  // chunk c of nc (past the end: the last one again)
+  __device__ __forceinline__ void load(u32x4 (&q)[NB], int c, int nc) const {
+    c = min(c, nc - 1);
+    const int at = c * 64 + (c == nc - 1 ? tail : 0);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) q[j] = *(const u32x4*)(p[j] + at);
   }
 };
 
@@ -212,31 +233,19 @@ __device__ __forceinline__ u32x4 load_row(__amdgpu_buffer_rsrc_t x, int off, int
 // step with the next D in flight; each wave passes its part of the rows (4 RX
 // of them) through LDS of its own. The W sums meet in LDS, added in wave order.
 //
-// Scales and zero points of KB chunks at a time go to LDS first, 8 groups a
-// lane: read where they are used they cost a cache line look-up for every
-// lane (a 16 x 4096 x 11007 product with groups of 32: 128 of a chunk's 208).
-//
 // The loop has no branches around loads (a conditional load makes hipcc wait for
 // the loads after it as well): chunk numbers past the end repeat the last one and
 // are not computed; a partial last chunk reads weights from inside the column
 // and zeros for the rows.
-constexpr int KB = 64;
-
-template <int NB, int SG>
-struct ScaleBlock {  // [column][KB * SG groups], 8 bytes between columns against bank conflicts
-  static constexpr int NG = KB * SG, SP = 2 * NG + 8, ZP = NG + 8, BYTES = 16 * NB * (SP + ZP);
-  static constexpr int PIECES = 16 * NB * NG / 8;  // of 8 groups
-};
 
 template <int NB, int RX>
 struct Step {
   u32x4 q[NB], x[RX];
 };
 
-template <int DT, int NB, int SG, int RX, bool ZERO>
+template <int DT, int NB, int SG, int RX, bool ZERO, class SB>
 __device__ __forceinline__ void multiply(f32x4 (&acc)[NB], Step<NB, RX>& b, const Bits& bits, char* xl, const char* sl,
                                          int at, int lane) {
-  using SB = ScaleBlock<NB, SG>;
   constexpr int PER = 4 / SG;  // MFMAs of a group
   const int l16 = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -244,11 +253,10 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[NB], Step<NB, RX>& b, cons
     const int row = 4 * i + g;  // piece l16 of it
     *(lds_u32x4_t*)(xl + row * 256 + ((l16 ^ row) << 4)) = __builtin_bit_cast(u32x4, permute_row(b.x[i]));
   }
-  Scales<DT, SG, 1, ZERO> sc[NB];
+  Scales<SG, DT, ZERO> sc[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int c = 16 * j + l16;
-    sc[j].load_lds(sl + c * SB::SP + 2 * at, sl + 16 * NB * SB::SP + c * SB::ZP + at);
+    SB::read(sc[j], sl, 16 * j + l16, at);
     to_operand(b.q[j], (l16 * 4 + g) * 4);
   }
   f32x4 p[NB];
@@ -281,7 +289,8 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[NB], Step<NB, RX>& b, cons
 
 template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
 __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
-  using SB = ScaleBlock<NB, SG>;
+  constexpr int KB = 64;  // chunks whose scales are in LDS
+  using SB = ScaleBlock<DT, 16 * NB, SG, KB, ZERO, 64 * W>;
   constexpr int XL = 4096, XS = W * (NB > 4 ? NB * 1024 : XL);  // a wave's rows of a chunk; later its sums
   static_assert(NB <= 4, "the sums reuse the rows' LDS");
   __shared__ __attribute__((aligned(1024))) char smem[XS + SB::BYTES];
@@ -311,10 +320,7 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
   if (nc > 0) {
     const int part = a.K % 128;  // k of a partial last chunk
     const long long first = (long long)r.e * a.N;
-    const unsigned char* q[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-      q[j] = (const unsigned char*)a.B + (first + min(n0 + 16 * j + (lane >> 2), a.N - 1)) * (a.K / 2) + 16 * (lane & 3);
+    const Weights<NB> q(a, first, n0, lane);
     const __amdgpu_buffer_rsrc_t xr = rows_buffer(a, r);
     int xo[RX], xt[RX];  // row offsets, and those of the last chunk
 #pragma unroll
@@ -322,17 +328,14 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
       xo[i] = 4 * i + g < r.rows ? (4 * i + g) * (int)a.lda * 2 + 16 * l16 : kOutside;
       xt[i] = part && 8 * l16 >= part ? kOutside : xo[i];
     }
-    const int qt = part ? min(16 * (lane & 3), part / 2 - 16) - 16 * (lane & 3) : 0;
 #pragma unroll
     for (int i = RX * 4 + g; i < 16; i += 4)  // rows that there are not
       *(lds_u32x4_t*)(xl + i * 256 + (l16 << 4)) = u32x4{0u, 0u, 0u, 0u};
     const Bits bits = Bits::make<DT>();
 
     auto load = [&](Step<NB, RX>& b, int c) {
+      q.load(b.q, c, nc);
       c = min(c, nc - 1);
-      const int at = c * 64 + (c == nc - 1 ? qt : 0);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) b.q[j] = *(const u32x4*)(q[j] + at);
 #pragma unroll
       for (int i = 0; i < RX; ++i) b.x[i] = load_row(xr, c == nc - 1 ? xt[i] : xo[i], c * 256);
     };
@@ -342,48 +345,17 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
       const int g0 = SG > 1 ? k0 * SG : group_of(a, k0);
       int c = k0 + w * per;
       const int end = min(k0 + kn, c + per);
-      // this block's scales, 8 groups a lane; what is not there is zero
-      constexpr int CH = (SB::PIECES + 64 * W - 1) / (64 * W);
-      u32x4 sv[CH];
-      u32x2 zv[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int at = tid + i * 64 * W, col = at / (SB::NG / 8), gr = g0 + at % (SB::NG / 8) * 8;
-        const long long off = (first + min(n0 + col, a.N - 1)) * a.groups + gr;
-        const unsigned short* sp = (const unsigned short*)a.scale + off;
-        const unsigned char* zp = a.zero + off;
-        sv[i] = u32x4{0u, 0u, 0u, 0u};
-        zv[i] = u32x2{0u, 0u};
-        if (gr + 8 <= a.groups) {
-          __builtin_memcpy(&sv[i], sp, 16);
-          if constexpr (ZERO) __builtin_memcpy(&zv[i], zp, 8);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 7; ++t)
-            if (gr + t < a.groups) {
-              sv[i][t >> 1] |= (unsigned)sp[t] << (16 * (t & 1));
-              if constexpr (ZERO) zv[i][t >> 2] |= (unsigned)zp[t] << (8 * (t & 3));
-            }
-        }
-      }
+      SB sb;
+      sb.load(a, first, n0, g0, tid);
       Step<NB, RX> st[D];
 #pragma unroll
       for (int d = 0; d < D; ++d) load(st[d], c + d);
       if (k0 > 0) __syncthreads();  // the block before is used up
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int at = tid + i * 64 * W, col = at / (SB::NG / 8), gr = at % (SB::NG / 8) * 8;
-        if (SB::PIECES % (64 * W) == 0 || at < SB::PIECES) {
-          char* p = sl + col * SB::SP + 2 * gr;
-          *(lds_u32x2*)p = u32x2{sv[i][0], sv[i][1]};
-          *(lds_u32x2*)(p + 8) = u32x2{sv[i][2], sv[i][3]};
-          if constexpr (ZERO) *(lds_u32x2*)(sl + 16 * NB * SB::SP + col * SB::ZP + gr) = zv[i];
-        }
-      }
+      sb.store(sl, tid);
       __syncthreads();
       auto mul = [&](Step<NB, RX>& b, int c) {
         const int at = SG > 1 ? (c - k0) * SG : group_of(a, c) - g0;
-        multiply<DT, NB, SG, RX, ZERO>(acc, b, bits, xl, sl, at, lane);
+        multiply<DT, NB, SG, RX, ZERO, SB>(acc, b, bits, xl, sl, at, lane);
       };
       for (int left = (per + D - 1) / D; left > 1; --left, c += D) {
 #pragma unroll
@@ -417,20 +389,22 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
 }
 
 // ---- more rows -----------------------------------------------------------
-// A workgroup takes 16 MB rows x 64 NB columns: 4 column waves of 16 NB
-// columns, twice, for the even and the odd chunks of k. The rows of both chunks
-// are staged through LDS, permuted on the way in ([row][256 B], 16-B piece c
-// at c ^ (row & 15): conflict-free both ways), the next pair in registers
+// A workgroup takes 16 MB rows x 64 NB columns: 4 column waves of 16 NB columns for
+// each of KW parts of k (every KW-th chunk). The rows of KW chunks are staged through LDS, permuted on the way in ([row][256 B], 16-B piece c
+// at c ^ (row & 15): conflict-free both ways), the next ones in registers
 // meanwhile. In bf16 a group's correction (16 + zero) * (sum of x) takes the
 // sum from one product with ones for all of a wave's columns.
-template <int DT, int MB, int NB, int SG, bool ZERO>
-__global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
+template <int DT, int MB, int NB, int SG, bool ZERO, int KW>
+__global__ void __launch_bounds__(256 * KW) gemm_int4_rows(Args a) {
   constexpr int BM = 16 * MB, BN = 64 * NB, XB = BM * 256;  // bytes of a chunk's rows
-  constexpr int CH = 2 * XB / 16 / 512;                     // 16-B pieces a thread stages
-  constexpr int RED = 4 * 64 * MB * NB * 4 * 4;
-  constexpr int LDS = 4 * XB > RED ? 4 * XB : RED;
-  static_assert(CH * 512 * 16 == 2 * XB, "whole pieces");
-  __shared__ __attribute__((aligned(1024))) char smem[LDS];
+  constexpr int THREADS = 256 * KW;
+  constexpr int CH = XB / 16 / 256;                         // 16-B pieces a thread stages
+  constexpr int XS = 2 * KW * XB;
+  static_assert((KW - 1) * 4 * 64 * MB * NB * 16 <= XS, "the sums reuse the rows' LDS");
+  constexpr int KB = 32;  // chunks whose scales are in LDS
+  using SB = ScaleBlock<DT, BN, SG, KB, ZERO, THREADS>;
+  static_assert(CH * 256 * 16 == XB, "whole pieces");
+  __shared__ __attribute__((aligned(1024))) char smem[XS + SB::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wc = w & 3, half = w >> 2;
   const int l16 = lane & 15, g = lane >> 4;
@@ -450,7 +424,9 @@ __global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
   }
   const int n0 = tn * BN + wc * (16 * NB);
   const int K = r.e == a.E ? 0 : a.K;  // rows behind the last group: zeros
-  const Columns<NB> cols(a, r.e == a.E ? 0 : r.e, n0, lane);
+  const long long first = (long long)(r.e == a.E ? 0 : r.e) * a.N;
+  const Weights<NB> weights(a, first, n0, lane);
+  char* sl = smem + XS;
   const __amdgpu_buffer_rsrc_t xr = rows_buffer(a, r);
 
   f32x4 acc[MB][NB];
@@ -459,60 +435,68 @@ __global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int np = (K + 255) / 256;  // pairs of chunks
+  const int nc = (K + 127) / 128, np = (nc + KW - 1) / KW;  // chunks, and steps of KW
   const Bits bits = Bits::make<DT>();
-  u32x4 xs[CH], q[NB], qn[NB];
-  Scales<DT, SG, 1, ZERO> s[NB], sn[NB];
+  u32x4 xs[CH], qn[NB], q[NB];
   int xo[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int at = tid + i * 512, row = at >> 5;
-    xo[i] = row < r.rows ? (row * (int)a.lda + (at & 31) * 8) * 2 : kOutside;
+    const int at = tid + i * THREADS, row = at / (16 * KW);
+    xo[i] = row < r.rows ? (row * (int)a.lda + at % (16 * KW) * 8) * 2 : kOutside;
   }
-  auto load_rows = [&](int pair) {
-    const int left = K - pair * 256;
+  // Rows and weights of a step (rows past K are zeros, weights repeat the last chunk)
+  auto load = [&](int step) {
+    weights.load(qn, KW * step + half, nc);
+    const int left = K - step * (128 * KW);
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      xs[i] = load_row(xr, (tid & 31) * 8 < left ? xo[i] : kOutside, pair * 512);
+      xs[i] = load_row(xr, tid % (16 * KW) * 8 < left ? xo[i] : kOutside, left > 0 ? step * (256 * KW) : 0);
   };
-  // (k past the end: any weight, the rows are zero there)
-  auto load_weight = [&](int pair) {
-    const int c = 2 * pair + half, s0 = SG > 1 ? c * SG : group_of(a, c);
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int piece = 16 * (lane & 3);
-      qn[j] = *(const u32x4*)(cols.q[j] - piece + min(c * 64 + piece, K / 2 - 16));
-      if (SG == 1 || s0 + SG <= a.groups) sn[j].load(cols.s[j] + min(s0, a.groups - 1), cols.z[j] + min(s0, a.groups - 1));
-      else sn[j].load_part(cols.s[j] + min(s0, a.groups - 1), cols.z[j] + min(s0, a.groups - 1), max(a.groups - s0, 1));
-    }
-  };
-  if (np > 0) {
-    load_rows(0);
-    load_weight(0);
-  }
-  for (int pair = 0; pair < np; ++pair) {
-    char* buf = smem + (pair & 1) * 2 * XB;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int at = tid + i * 512, row = at >> 5, c = at & 31;
-      *(lds_u32x4_t*)(buf + (c >> 4) * XB + row * 256 + (((c & 15) ^ (row & 15)) << 4)) =
-          __builtin_bit_cast(u32x4, permute_row(xs[i]));
-    }
+  // Rows to LDS, weights to the operand's lanes: what the next step will use
+  auto ready = [&](int step) {
+    char* buf = smem + (step & 1) * KW * XB;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       q[j] = qn[j];
-      s[j] = sn[j];
+      to_operand(q[j], (l16 * 4 + g) * 4);
     }
-    if (pair + 1 < np) {
-      load_rows(pair + 1);
-      load_weight(pair + 1);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int at = tid + i * THREADS, row = at / (16 * KW), c = at % (16 * KW);
+      *(lds_u32x4_t*)(buf + (c >> 4) * XB + row * 256 + (((c & 15) ^ (row & 15)) << 4)) =
+          __builtin_bit_cast(u32x4, permute_row(xs[i]));
     }
-    __syncthreads();  // this buffer is written; the other one's readers are done
-    const char* xb = buf + half * XB;
+  };
+  if (np > 0) {
+    load(0);
+    ready(0);
+    load(1);
+  }
+  int g0 = 0;
+  for (int step = 0; step < np; ++step) {
+    if (step % (KB / KW) == 0) {  // the scales of the next KB chunks
+      g0 = SG > 1 ? KW * step * SG : group_of(a, KW * step);
+      SB sb;
+      sb.load(a, first, tn * BN, g0, tid);
+      if (step) __syncthreads();  // those before are used up
+      sb.store(sl, tid);
+    }
+    // this step's rows are written, and the other buffer's readers are done (loads stay in flight)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const char* xb = smem + (step & 1) * KW * XB + half * XB;
+    u32x4 qc[NB];
+    Scales<SG, DT, ZERO> s[NB];
+    const int c = min(KW * step + half, nc - 1), at = SG > 1 ? c * SG - g0 : group_of(a, c) - g0;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      SB::read(s[j], sl, wc * (16 * NB) + 16 * j + l16, at);
+      qc[j] = q[j];
+    }
+    // the next step's rows and operands, beside this one's products
+    ready(step + 1);
+    load(step + 2);
     constexpr int PER = 4 / SG;
     f32x4 p[MB][NB], px[MB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) to_operand(q[j], (l16 * 4 + g) * 4);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       s16x8 xf[MB];
@@ -530,7 +514,7 @@ __global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const unsigned z = s[j].zero(t / PER);
-        const s16x8 wf = widen<DT, true>(q[j][t], bits, minus_of<DT>(z));
+        const s16x8 wf = widen<DT, true>(qc[j][t], bits, minus_of<DT>(z));
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           if (t % PER == 0) p[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -550,16 +534,17 @@ __global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
     }
   }
 
-  // odd chunks' sums to the even chunks' waves
+  // the other K parts' sums to the first one's waves, added in order
   __syncthreads();
   float* red = (float*)smem + wc * (MB * NB * 256) + lane;
-  if (half == 1) {
+  if (half > 0) {
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) red[((i * NB + j) * 4 + v) * 64] = acc[i][j][v];
+        for (int v = 0; v < 4; ++v)
+          red[(half - 1) * (MB * NB * 1024) + ((i * NB + j) * 4 + v) * 64] = acc[i][j][v];
   }
   __syncthreads();
   if (half == 0) {
@@ -569,10 +554,12 @@ __global__ void __launch_bounds__(512) gemm_int4_rows(Args a) {
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
+          float sum = acc[i][j][v];
+#pragma unroll
+          for (int u = 0; u < KW - 1; ++u) sum += red[u * (MB * NB * 1024) + ((i * NB + j) * 4 + v) * 64];
           const int m = 16 * i + 4 * g + v, n = n0 + 16 * j + l16;
           if (m < r.rows && n < a.N)
-            ((unsigned short*)a.C)[((long long)r.row0 + m) * a.ldc + n] =
-                (unsigned short)pack2<DT>(acc[i][j][v] + red[((i * NB + j) * 4 + v) * 64], 0.f);
+            ((unsigned short*)a.C)[((long long)r.row0 + m) * a.ldc + n] = (unsigned short)pack2<DT>(sum, 0.f);
         }
   }
 }
@@ -593,12 +580,12 @@ hipError_t launch_few(Args a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int DT, int MB, int NB, int SG, bool ZERO>
+template <int DT, int MB, int NB, int SG, bool ZERO, int KW>
 hipError_t launch_rows(Args a, hipStream_t s) {
   a.tiles_n = (a.N + 64 * NB - 1) / (64 * NB);
   const long long blocks = blocks_of(a, 16 * MB, 64 * NB);
   if (blocks > (1ll << 30)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((gemm_int4_rows<DT, MB, NB, SG, ZERO>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(512), 0, s,
+  hipLaunchKernelGGL((gemm_int4_rows<DT, MB, NB, SG, ZERO, KW>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(256 * KW), 0, s,
                      a);
   return hipGetLastError();
 }
@@ -620,9 +607,9 @@ hipError_t pick(const Args& a, hipStream_t s) {
   const int avg = (a.T + a.E - 1) / a.E;
   if (a.T <= 4) return pick_few<DT, SG, 1, ZERO>(a, s);
   if (avg <= 16) return pick_few<DT, SG, 4, ZERO>(a, s);
-  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO>(a, s);
-  if (blocks_of(a, 64, 128) >= 512) return launch_rows<DT, 4, 2, SG, ZERO>(a, s);
-  return launch_rows<DT, 4, 1, SG, ZERO>(a, s);
+  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO, 2>(a, s);
+  if (blocks_of(a, 64, 128) >= 512) return launch_rows<DT, 4, 2, SG, ZERO, 2>(a, s);
+  return launch_rows<DT, 4, 1, SG, ZERO, 2>(a, s);
 }
 
 template <int DT, bool ZERO>
