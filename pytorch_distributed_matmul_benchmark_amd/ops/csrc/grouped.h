@@ -70,14 +70,35 @@ __device__ __forceinline__ LaneGroup lane_group(const GroupArgs& a, int c0, int 
   return l;
 }
 
-// The group's tile that L of the launch's row-tile x column-tile products
-// falls to. Every wave of the workgroup searches by itself (no barrier): a
-// lane takes a group, a 64-lane prefix sum gives the tiles before it; more
-// than 64 groups go by 64 a pass. Returns false where block b has no tile.
-//
-// Order: products are dealt to the XCDs (blocks b and b + 8 share one) in
-// runs of up to 32, so that an XCD's 32 CUs work on 8 row tiles x 4 column
-// tiles and its L2 serves each operand panel to several of them.
+// Number of the row tile x column tile product that block b works on, of total x
+// tiles_n; false where it has none. Products are dealt to the XCDs (blocks b and b
+// + 8 share one) in runs of up to 32, so that an XCD's 32 CUs work on 8 row tiles
+// x 4 column tiles and its L2 serves each operand panel to several of them.
+__device__ __forceinline__ bool product_of(unsigned total, unsigned tiles_n, unsigned b, int& slot, int& tn) {
+  const unsigned prods = total * tiles_n;
+  const unsigned per = (prods + 7) / 8, x = b & 7, i = b >> 3;
+  if (i >= per) return false;
+  const unsigned full = per / 32 * 32;
+  const unsigned L = i < full ? (i / 32) * 256 + x * 32 + i % 32 : full * 8 + x * (per - full) + (i - full);
+  if (L >= prods) return false;
+  const unsigned sg = L / (8u * tiles_n), s0 = sg * 8;
+  const unsigned gm = min(8u, total - s0), rem = L - sg * 8u * tiles_n;
+  tn = (int)(rem / gm);
+  slot = (int)(s0 + rem % gm);
+  return true;
+}
+
+// The tile that `slot` of the groups in l is, `base` slots before them; inc: prefix sums of l.tiles.
+template <int BM>
+__device__ __forceinline__ RowTile pick_tile(const LaneGroup& l, int inc, int slot, int base, int c0) {
+  const int k = __builtin_ctzll(__ballot(slot < base + inc));  // first lane whose tiles reach slot
+  const int off = (slot - base - __builtin_amdgcn_readlane(inc, k) + __builtin_amdgcn_readlane(l.tiles, k)) * BM;
+  return RowTile{c0 + k, __builtin_amdgcn_readlane(l.lo, k) + off, min(BM, __builtin_amdgcn_readlane(l.n, k) - off)};
+}
+
+// Block b's tile. Every wave of the workgroup searches by itself (no barrier): a
+// lane takes a group, a 64-lane prefix sum gives the tiles before it; more than
+// 64 groups go by 64 a pass.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int lane, RowTile& r, int& tn) {
   int carry = 0;
@@ -86,17 +107,8 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int la
   int total = __builtin_amdgcn_readlane(inc, 63);
   for (int c0 = 64; c0 < a.E + 1; c0 += 64)  // (the tail counts as a group)
     total += __builtin_amdgcn_readlane(wave_scan(lane_group<BM>(a, c0, lane, carry).tiles), 63);
-  // XCD-run order over `total` x tiles_n products
-  const unsigned prods = (unsigned)total * (unsigned)a.tiles_n;
-  const unsigned per = (prods + 7) / 8, x = b & 7, i = b >> 3;
-  if (i >= per) return false;
-  const unsigned full = per / 32 * 32;
-  const unsigned L = i < full ? (i / 32) * 256 + x * 32 + i % 32 : full * 8 + x * (per - full) + (i - full);
-  if (L >= prods) return false;
-  const unsigned sg = L / (8u * a.tiles_n), s0 = sg * 8;
-  const unsigned gm = min(8u, (unsigned)total - s0), rem = L - sg * 8u * a.tiles_n;
-  tn = (int)(rem / gm);
-  const int slot = (int)(s0 + rem % gm);
+  int slot;
+  if (!product_of((unsigned)total, (unsigned)a.tiles_n, b, slot, tn)) return false;
   int base = 0, c0 = 0;
   for (;;) {
     const int tot = __builtin_amdgcn_readlane(inc, 63);
@@ -107,13 +119,7 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int la
     l = lane_group<BM>(a, c0, lane, carry);
     inc = wave_scan(l.tiles);
   }
-  const unsigned long long at = __ballot(slot < base + inc);  // first lane whose tiles reach slot
-  const int k = __builtin_ctzll(at);
-  const int before = base + __builtin_amdgcn_readlane(inc, k) - __builtin_amdgcn_readlane(l.tiles, k);
-  const int off = (slot - before) * BM;
-  r.e = c0 + k;
-  r.row0 = __builtin_amdgcn_readlane(l.lo, k) + off;
-  r.rows = min(BM, __builtin_amdgcn_readlane(l.n, k) - off);
+  r = pick_tile<BM>(l, inc, slot, base, c0);
   return true;
 }
 

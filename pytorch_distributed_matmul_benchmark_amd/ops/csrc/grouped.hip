@@ -369,7 +369,7 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
   a.zero_tail = p.zero_tail;
   const bool buf = buf_ok(p.A, p.lda, 0, es) && buf_ok(p.B, p.ldb, p.sB, es);
   const int avg = (p.T + p.E - 1) / p.E;
-  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 96) && (red || p.K > 0) &&
+  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 96) &&
       grouped_w4_ok(a, red, p.b_colmajor))
     return grouped_w4(a, p.dtype, red, p.b_colmajor, stream);
   switch (p.dtype) {

@@ -48,5 +48,7 @@ def test_hazards(src):
 def test_counted_waits_stay_countable():
     """grouped_w4's K-loop waits on counts of vector-memory operations in flight, at most 63."""
     for name, body in mfma._kernels(_asm("grouped_w4.hip")):
-        loop_end = body.rfind("s_waitcnt vmcnt(0)")
-        assert peak_outstanding(body[:loop_end]) <= MAX, name
+        first = re.search(r"buffer_load_dwordx4 .* lds", body).start()  # all before it has been waited for
+        assert "s_waitcnt vmcnt(0)" in body[:first]
+        peak = peak_outstanding(body[first:body.rfind("s_waitcnt vmcnt(0)")])
+        assert 48 < peak <= MAX, (name, peak)
