@@ -27,6 +27,8 @@
 #include "api.h"
 #include "grouped.h"
 
+#include <cmath>
+
 namespace pdmb {
 namespace kgrp {
 
@@ -284,6 +286,34 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
     }
   }
 
+  // Whole 16-byte pieces of C go out as rows through this wave's part of the LDS: stored
+  // from the accumulators, a row's 32 bytes at a time, a weight gradient of 48 experts
+  // of 167 rows, 2048 x 1024, takes 113 us instead of 80.
+  constexpr int ROWB = NB * 16 * ES, PITCH = ROWB + 16, LPR = ROWB / 16, RPI = 64 / LPR;
+  static_assert(4 * 16 * PITCH <= 2 * STAGE && 16 % RPI == 0, "epilogue rows");
+  if ((uintptr_t)a.C % 16 == 0 && a.ldc * ES % 16 == 0 && a.sC * ES % 16 == 0 && a.N * ES % 16 == 0) {
+    typedef __attribute__((address_space(3))) char lds_char;
+    lds_char* eb = (lds_char*)(lds_void*)(smem + w * 16 * PITCH);
+    __syncthreads();  // the last K-tile is read
+    const int rl = lane / LPR, cb = lane % LPR * 16;
+    const bool in = wc * ROWB + cb < cols * ES;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        lds_char* p = eb + l16 * PITCH + (j * 16 + 4 * g) * ES;
+        if constexpr (DT == kF32) *(__attribute__((address_space(3))) f32x4*)p = acc[i][j];
+        else *(lds_u32x2*)p = u32x2{pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3])};
+      }
+#pragma unroll
+      for (int r = 0; r < 16 / RPI; ++r) {
+        const u32x4 x = *(lds_u32x4_t*)(eb + (r * RPI + rl) * PITCH + cb);
+        const int row = wr * (BM / WR) + i * 16 + r * RPI + rl;
+        if (in && row < rows) __builtin_nontemporal_store(x, (u32x4*)(Cp + row * a.ldc * ES + wc * ROWB + cb));
+      }
+    }
+    return;
+  }
   const bool whole = (uintptr_t)a.C % (4 * ES) == 0 && a.ldc % 4 == 0 && a.sC % 4 == 0;
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
@@ -312,8 +342,29 @@ hipError_t launch(GroupArgs a, bool buf, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Row tiles of BM rows that T rows of E groups make, on average: every second
+// group's last tile counts, and no group with rows goes without one.
+inline double row_tiles(const GroupArgs& a, int bm) {
+  const double t = (double)a.T / bm + 0.5 * a.E;
+  const double least = a.T < a.E ? a.T : a.E;
+  return t > least ? t : least;
+}
+
+// Microseconds of 64 k in 16 bits of `tiles` tiles: one where the CUs hold no second one, full
+// where they hold `per` of them (measured: 256 x 256 tiles of grouped_w4.hip 1.5 us a
+// round of 256; 128 x 128 alone 0.87, two a CU 1.83; 64 x 128 alone 0.6, three a CU 1.8).
+// So 48 experts of 167 rows, 2048 x 1024, run on large tiles (58 us; 128 rows 80),
+// of 43 rows on 64 (46; large ones 51), and 4 experts of 200 rows, where large tiles
+// leave most CUs idle, on 64 as well (19; 128 rows 28, large ones 43).
+inline double tile_time(double tiles, double alone, double full, int per) {
+  if (tiles <= 256) return alone;
+  const double t = full * tiles / (256.0 * per);
+  return t > alone ? t : alone;
+}
+inline double large_time(double tiles) { return 1.5 * ceil(tiles / 256.0); }
+
 template <int DT, bool B_KC>
-hipError_t launch_rows(const GroupArgs& a, bool buf, hipStream_t s) {
+hipError_t launch_rows(const GroupArgs& a, bool buf, bool large, hipStream_t s) {
   // Rows a group has on average: a tile taller than that computes rows that
   // no group has, one shorter reads the weights once more for each tile.
   const int avg = (a.T + a.E - 1) / a.E;
@@ -326,15 +377,31 @@ hipError_t launch_rows(const GroupArgs& a, bool buf, hipStream_t s) {
     return launch<DT, false, B_KC, 64, 64, 2, 2>(a, buf, s);
   } else {
     if (avg <= 32) return launch<DT, false, B_KC, 32, 128, 1, 1>(a, buf, s);
-    if (avg <= 64) return launch<DT, false, B_KC, 64, 128, 2, 1>(a, buf, s);
+    const int n256 = (a.N + 255) / 256, n128 = (a.N + 127) / 128;
+    const double t64 = tile_time(row_tiles(a, 64) * n128, 0.6, 1.8, 3);
+    const double t128 = tile_time(row_tiles(a, 128) * n128, 0.87, 1.83, 2);
+    if (large && large_time(row_tiles(a, 256) * n256) <= (t64 < t128 ? t64 : t128))
+      return grouped_w4(a, DT, false, B_KC, s);
+    if (t64 < t128) return launch<DT, false, B_KC, 64, 128, 2, 1>(a, buf, s);
     return launch<DT, false, B_KC, 128, 128, 2, 1>(a, buf, s);
   }
 }
 
 template <int DT>
-hipError_t launch_reduce(const GroupArgs& a, bool buf, hipStream_t s) {
-  if constexpr (DT == kF32) return launch<DT, true, false, 64, 64, 2, 2>(a, buf, s);
-  return launch<DT, true, false, 128, 128, 2, 1>(a, buf, s);
+hipError_t launch_reduce(const GroupArgs& a, bool buf, bool large, hipStream_t s) {
+  if constexpr (DT == kF32) {
+    return launch<DT, true, false, 64, 64, 2, 2>(a, buf, s);
+  } else {
+    // As above, with what a tile costs beside its 64-k steps: large ones 5 us, 128 x 128
+    // 1.5 (3 alone). (48 experts of 167 rows, 2048 x 1024: large 66 us, 128 rows 80; 64 experts of
+    // 32 rows: 82, 60; 16 of 512: 43, 58.)
+    const double nk = ((double)a.T / a.E + 63) / 64, even = nk < 4 ? 4 : nk + 1;
+    const double t256 = (double)a.E * ((a.M + 255) / 256) * ((a.N + 255) / 256);
+    const double t128 = (double)a.E * ((a.M + 127) / 128) * ((a.N + 127) / 128);
+    const double small = t128 <= 256 ? 0.87 * nk + 3 : (1.83 * nk + 1.5) * (t128 <= 512 ? 1.0 : t128 / 512);
+    if (large && (1.5 * even + 5) * ceil(t256 / 256) <= small) return grouped_w4(a, DT, true, false, s);
+    return launch<DT, true, false, 128, 128, 2, 1>(a, buf, s);
+  }
 }
 
 }  // namespace kgrp
@@ -368,23 +435,20 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
   a.sC = p.sC;
   a.zero_tail = p.zero_tail;
   const bool buf = buf_ok(p.A, p.lda, 0, es) && buf_ok(p.B, p.ldb, p.sB, es);
-  const int avg = (p.T + p.E - 1) / p.E;
-  if (p.dtype != kF32 && (red ? p.M >= 256 && p.N >= 256 : avg >= 96) &&
-      grouped_w4_ok(a, red, p.b_colmajor))
-    return grouped_w4(a, p.dtype, red, p.b_colmajor, stream);
+  const bool large = p.dtype != kF32 && grouped_w4_ok(a, red, p.b_colmajor);
   switch (p.dtype) {
     case kF32:
-      return red            ? kgrp::launch_reduce<kF32>(a, buf, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kF32, true>(a, buf, stream)
-                            : kgrp::launch_rows<kF32, false>(a, buf, stream);
+      return red            ? kgrp::launch_reduce<kF32>(a, buf, large, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kF32, true>(a, buf, large, stream)
+                            : kgrp::launch_rows<kF32, false>(a, buf, large, stream);
     case kF16:
-      return red            ? kgrp::launch_reduce<kF16>(a, buf, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kF16, true>(a, buf, stream)
-                            : kgrp::launch_rows<kF16, false>(a, buf, stream);
+      return red            ? kgrp::launch_reduce<kF16>(a, buf, large, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kF16, true>(a, buf, large, stream)
+                            : kgrp::launch_rows<kF16, false>(a, buf, large, stream);
     case kBF16:
-      return red            ? kgrp::launch_reduce<kBF16>(a, buf, stream)
-             : p.b_colmajor ? kgrp::launch_rows<kBF16, true>(a, buf, stream)
-                            : kgrp::launch_rows<kBF16, false>(a, buf, stream);
+      return red            ? kgrp::launch_reduce<kBF16>(a, buf, large, stream)
+             : p.b_colmajor ? kgrp::launch_rows<kBF16, true>(a, buf, large, stream)
+                            : kgrp::launch_rows<kBF16, false>(a, buf, large, stream);
     default:
       return hipErrorInvalidValue;
   }
