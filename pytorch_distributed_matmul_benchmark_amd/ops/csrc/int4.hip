@@ -87,12 +87,12 @@ __device__ __forceinline__ Minus minus_of(unsigned z) {
                      : Minus{{z * 0x00010001u + 0xe400e400u, z * 0x00100010u + 0xd400d400u}};
 }
 
-// 8 nibbles as B + q (bf16; EVEN: B = 16 for all), or as q - zero (fp16).
-template <int DT, bool EVEN = false>
+// 8 nibbles as B + q (bf16), or as q - zero (fp16).
+template <int DT>
 __device__ __forceinline__ s16x8 widen(unsigned d, const Bits& b, const Minus& minus) {
   u32x4 v;
   if constexpr (DT == kBF16) {
-    v = u32x4{EVEN ? ((d << 3) & b.mask1) | b.or1 : (d & b.mask0) | b.or0, ((d >> 1) & b.mask1) | b.or1, ((d >> 5) & b.mask1) | b.or1,
+    v = u32x4{(d & b.mask0) | b.or0, ((d >> 1) & b.mask1) | b.or1, ((d >> 5) & b.mask1) | b.or1,
               ((d >> 9) & b.mask1) | b.or1};
   } else {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -145,7 +145,7 @@ struct Scales {
 template <int DT, int COLS, int SG, int KB, bool ZERO, int THREADS>
 struct ScaleBlock {
   static constexpr int NG = KB * SG, SP = 2 * NG + 8, ZP = NG + 8, BYTES = COLS * (SP + ZP);
-  static constexpr int PIECES = COLS * NG / 8, CH = (PIECES + THREADS - 1) / THREADS;
+  static constexpr int CHUNKS = KB, PIECES = COLS * NG / 8, CH = (PIECES + THREADS - 1) / THREADS;
   u32x4 s[CH];
   u32x2 z[CH];
   // groups from g0 of columns from n0 (of expert e's `first`); what is not there is zero
@@ -287,35 +287,11 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[NB], Step<NB, RX>& b, cons
   }
 }
 
-template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
-__global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
-  constexpr int KB = 64;  // chunks whose scales are in LDS
-  using SB = ScaleBlock<DT, 16 * NB, SG, KB, ZERO, 64 * W>;
-  constexpr int XL = 4096, XS = W * (NB > 4 ? NB * 1024 : XL);  // a wave's rows of a chunk; later its sums
-  static_assert(NB <= 4, "the sums reuse the rows' LDS");
-  __shared__ __attribute__((aligned(1024))) char smem[XS + SB::BYTES];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l16 = lane & 15, g = lane >> 4;
-
-  RowTile r;
-  int tn;
-  if (a.ends) {
-    if (!find_tile<16>(a, blockIdx.x, lane, r, tn)) return;
-  } else {
-    tn = blockIdx.x % a.tiles_n;
-    r.e = 0;
-    r.row0 = blockIdx.x / a.tiles_n * 16;
-    r.rows = min(16, a.T - r.row0);
-    if (r.rows <= 0) return;
-  }
-  const int n0 = tn * (16 * NB);
-  char* xl = smem + w * XL;
-  char* sl = smem + XS;
-  f32x4 acc[NB];
-#pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+// The wave's part of a tile's sums: 16 NB columns from n0, its run of k.
+template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D, class SB>
+__device__ __forceinline__ void few_sums(const Args& a, const RowTile& r, int n0, int tid, int w, char* xl, char* sl,
+                                         f32x4 (&acc)[NB]) {
+  const int lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int nc = r.e == a.E ? 0 : (a.K + 127) / 128;  // (rows behind the last group: zeros)
   if (nc > 0) {
     const int part = a.K % 128;  // k of a partial last chunk
@@ -340,8 +316,8 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
       for (int i = 0; i < RX; ++i) b.x[i] = load_row(xr, c == nc - 1 ? xt[i] : xo[i], c * 256);
     };
 
-    for (int k0 = 0; k0 < nc; k0 += KB) {
-      const int kn = min(KB, nc - k0), per = (kn + W - 1) / W;
+    for (int k0 = 0; k0 < nc; k0 += SB::CHUNKS) {
+      const int kn = min(SB::CHUNKS, nc - k0), per = (kn + W - 1) / W;
       const int g0 = SG > 1 ? k0 * SG : group_of(a, k0);
       int c = k0 + w * per;
       const int end = min(k0 + kn, c + per);
@@ -369,6 +345,37 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
         if (c + d < end) mul(st[d], c + d);
     }
   }
+}
+
+template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
+__global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
+  constexpr int KB = 64;  // chunks whose scales are in LDS
+  using SB = ScaleBlock<DT, 16 * NB, SG, KB, ZERO, 64 * W>;
+  constexpr int XL = 4096, XS = W * (NB > 4 ? NB * 1024 : XL);  // a wave's rows of a chunk; later its sums
+  static_assert(NB <= 4, "the sums reuse the rows' LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[XS + SB::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  RowTile r;
+  int tn;
+  if (a.ends) {
+    if (!find_tile<16>(a, blockIdx.x, lane, r, tn)) return;
+  } else {
+    tn = blockIdx.x % a.tiles_n;
+    r.e = 0;
+    r.row0 = blockIdx.x / a.tiles_n * 16;
+    r.rows = min(16, a.T - r.row0);
+    if (r.rows <= 0) return;
+  }
+  const int n0 = tn * (16 * NB);
+  char* xl = smem + w * XL;
+  char* sl = smem + XS;
+  f32x4 acc[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  few_sums<DT, NB, SG, RX, ZERO, W, D, SB>(a, r, n0, tid, w, xl, sl, acc);
 
   float* red = (float*)smem;  // [wave][16 NB columns x 16 rows]
   __syncthreads();
@@ -392,8 +399,7 @@ __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
 // A workgroup takes 16 MB rows x 64 NB columns: 4 column waves of 16 NB columns for
 // each of KW parts of k (every KW-th chunk). The rows of KW chunks are staged through LDS, permuted on the way in ([row][256 B], 16-B piece c
 // at c ^ (row & 15): conflict-free both ways), the next ones in registers
-// meanwhile. In bf16 a group's correction (16 + zero) * (sum of x) takes the
-// sum from one product with ones for all of a wave's columns.
+// meanwhile.
 template <int DT, int MB, int NB, int SG, bool ZERO, int KW>
 __global__ void __launch_bounds__(256 * KW) gemm_int4_rows(Args a) {
   constexpr int BM = 16 * MB, BN = 64 * NB, XB = BM * 256;  // bytes of a chunk's rows
@@ -496,39 +502,34 @@ __global__ void __launch_bounds__(256 * KW) gemm_int4_rows(Args a) {
     ready(step + 1);
     load(step + 2);
     constexpr int PER = 4 / SG;
-    f32x4 p[MB][NB], px[MB];
+    f32x4 p[MB][NB];
+    Minus minus[NB];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       s16x8 xf[MB];
 #pragma unroll
       for (int i = 0; i < MB; ++i)
         xf[i] = *(const lds_s16x8*)(xb + (16 * i + l16) * 256 + (((4 * t + g) ^ l16) << 4));
-      if constexpr (DT == kBF16) {
-        const s16x8 ones = __builtin_bit_cast(s16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          if (t % PER == 0) px[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-          px[i] = mfma16x16x32<DT>(xf[i], ones, px[i]);
-        }
-      }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const unsigned z = s[j].zero(t / PER);
-        const s16x8 wf = widen<DT, true>(qc[j][t], bits, minus_of<DT>(z));
+        if (t % PER == 0) minus[j] = minus_of<DT>(s[j].zero(t / PER));
+        const s16x8 wf = widen<DT>(qc[j][t], bits, minus[j]);
+        const s16x8 mf = __builtin_bit_cast(s16x8, u32x4{minus[j].m[0], minus[j].m[1], minus[j].m[1], minus[j].m[1]});
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           if (t % PER == 0) p[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
           p[i][j] = mfma16x16x32<DT>(xf[i], wf, p[i][j]);
         }
+        if constexpr (DT == kBF16) {
+#pragma unroll
+          for (int i = 0; i < MB; ++i) p[i][j] = mfma16x16x32<DT>(xf[i], mf, p[i][j]);
+        }
         if (t % PER == PER - 1) {
-          const float sc = s[j].scale(t / PER), off = -16.0f - (float)z;
+          const float sc = s[j].scale(t / PER);
 #pragma unroll
           for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const float d = DT == kBF16 ? fmaf(off, px[i][v], p[i][j][v]) : p[i][j][v];
-              acc[i][j][v] = fmaf(sc, d, acc[i][j][v]);
-            }
+            for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(sc, p[i][j][v], acc[i][j][v]);
         }
       }
     }
@@ -607,9 +608,11 @@ hipError_t pick(const Args& a, hipStream_t s) {
   const int avg = (a.T + a.E - 1) / a.E;
   if (a.T <= 4) return pick_few<DT, SG, 1, ZERO>(a, s);
   if (avg <= 16) return pick_few<DT, SG, 4, ZERO>(a, s);
-  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO, 2>(a, s);
+  // (100 x 4096 x 8192, groups of 64: 64 rows in 4 parts of k 21.6 us, 2 parts 24.0; 32 rows 26;
+  // 512 rows: 128 columns 67 us, 64 72. 32 rows: 4 parts 14.2, 2 15.7.)
+  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO, 4>(a, s);
   if (blocks_of(a, 64, 128) >= 512) return launch_rows<DT, 4, 2, SG, ZERO, 2>(a, s);
-  return launch_rows<DT, 4, 1, SG, ZERO, 2>(a, s);
+  return launch_rows<DT, 4, 1, SG, ZERO, 4>(a, s);
 }
 
 template <int DT, bool ZERO>
