@@ -198,9 +198,10 @@ __device__ __forceinline__ void store4(char* p, const f32x4& v, int left, bool w
   }
 }
 
-// RED: `reduce` (A and B are both KS). BM x BN tile, WR x 4 / WR waves.
-template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, bool BUF>
-__global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
+// RED: `reduce` (A and B are both KS). BM x BN tile, WR x 4 / WR waves; KW > 1: KW such
+// sets of waves take every KW-th K-tile, and their sums meet in LDS, added in order.
+template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, bool BUF, int KW>
+__global__ void __launch_bounds__(NT * KW) gemm_grouped(GroupArgs a) {
   constexpr int ES = esize<DT>();
   using TA = Tile<DT, !RED, BM, BUF>;
   using TB = Tile<DT, B_KC, BN, BUF>;
@@ -208,10 +209,11 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
   constexpr int WC = 4 / WR;
   constexpr int MB = BM / WR / 16, NB = BN / WC / 16;
   constexpr int STAGE = TA::BYTES + TB::BYTES;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE * KW];
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x % NT, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = KW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
   const int wr = w / WC, wc = w % WC, l16 = lane & 15, g = lane >> 4;
 
   const char *Ap, *Bp;
@@ -255,19 +257,19 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
     u32x4 va[PF][TA::CH], vb[PF][TB::CH];
 #pragma unroll
     for (int d = 0; d < PF; ++d) {
-      ta.load(va[d], d * BK, tid);
-      tb.load(vb[d], d * BK, tid);
+      ta.load(va[d], (d * KW + kw) * BK, tid);
+      tb.load(vb[d], (d * KW + kw) * BK, tid);
     }
-    for (int t0 = 0; t0 < nk; t0 += PF) {
+    for (int t0 = 0; t0 * KW < nk; t0 += PF) {
 #pragma unroll
       for (int d = 0; d < PF; ++d) {
-        const int t = t0 + d;
-        if (PF > 1 && t >= nk) break;
-        char* st = smem + (t & 1) * STAGE;
-        ta.store(st, va[d], t * BK, tid);
-        tb.store(st + TA::BYTES, vb[d], t * BK, tid);
-        ta.load(va[d], (t + PF) * BK, tid);
-        tb.load(vb[d], (t + PF) * BK, tid);
+        const int t = t0 + d;  // K-tile t KW + kw (past the end: zeros)
+        if (PF > 1 && t * KW >= nk) break;
+        char* st = smem + (kw * 2 + (t & 1)) * STAGE;
+        ta.store(st, va[d], (t * KW + kw) * BK, tid);
+        tb.store(st + TA::BYTES, vb[d], (t * KW + kw) * BK, tid);
+        ta.load(va[d], ((t + PF) * KW + kw) * BK, tid);
+        tb.load(vb[d], ((t + PF) * KW + kw) * BK, tid);
         // this stage is written; the other one's readers are done (LDS only: loads stay in flight)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
@@ -286,6 +288,26 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
     }
   }
 
+  if constexpr (KW > 1) {
+    static_assert((KW - 1) * NT * MB * NB * 16 <= 2 * STAGE * KW, "the sums reuse the stages");
+    float* red = (float*)smem + tid;
+    __syncthreads();
+    if (kw > 0) {
+#pragma unroll
+      for (int i = 0; i < MB * NB * 4; ++i)
+        red[((kw - 1) * (MB * NB * 4) + i) * NT] = acc[i / (4 * NB)][i / 4 % NB][i % 4];
+    }
+    __syncthreads();
+    if (kw == 0) {
+#pragma unroll
+      for (int i = 0; i < MB * NB * 4; ++i)
+#pragma unroll
+        for (int u = 0; u < KW - 1; ++u)
+          acc[i / (4 * NB)][i / 4 % NB][i % 4] += red[(u * (MB * NB * 4) + i) * NT];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+  }
   // Whole 16-byte pieces of C go out as rows through this wave's part of the LDS: stored
   // from the accumulators, a row's 32 bytes at a time, a weight gradient of 48 experts
   // of 167 rows, 2048 x 1024, takes 113 us instead of 80.
@@ -294,7 +316,7 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
   if ((uintptr_t)a.C % 16 == 0 && a.ldc * ES % 16 == 0 && a.sC * ES % 16 == 0 && a.N * ES % 16 == 0) {
     typedef __attribute__((address_space(3))) char lds_char;
     lds_char* eb = (lds_char*)(lds_void*)(smem + w * 16 * PITCH);
-    __syncthreads();  // the last K-tile is read
+    if constexpr (KW == 1) __syncthreads();  // the last K-tile is read
     const int rl = lane / LPR, cb = lane % LPR * 16;
     const bool in = wc * ROWB + cb < cols * ES;
 #pragma unroll
@@ -328,7 +350,7 @@ __global__ void __launch_bounds__(NT) gemm_grouped(GroupArgs a) {
   }
 }
 
-template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF>
+template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, int KW = 1>
 hipError_t launch(GroupArgs a, bool buf, hipStream_t s) {
   a.tiles_m = (a.M + BM - 1) / BM;
   a.tiles_n = (a.N + BN - 1) / BN;
@@ -336,9 +358,11 @@ hipError_t launch(GroupArgs a, bool buf, hipStream_t s) {
                                : (row_tiles_bound(a.T, a.E, BM, a.zero_tail) * a.tiles_n + 7) / 8 * 8;
   if (blocks > (1ll << 30)) return hipErrorInvalidValue;
   if (buf)
-    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, PF, true>), dim3((unsigned)blocks), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, PF, true, KW>), dim3((unsigned)blocks), dim3(NT * KW), 0,
+                       s, a);
   else
-    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, false>), dim3((unsigned)blocks), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, false, KW>), dim3((unsigned)blocks), dim3(NT * KW), 0,
+                       s, a);
   return hipGetLastError();
 }
 
@@ -368,7 +392,17 @@ hipError_t launch_rows(const GroupArgs& a, bool buf, bool large, hipStream_t s) 
   // Rows a group has on average: a tile taller than that computes rows that
   // no group has, one shorter reads the weights once more for each tile.
   const int avg = (a.T + a.E - 1) / a.E;
-  if (avg <= 16) return launch<DT, false, B_KC, 16, 128, 1, 1>(a, buf, s);
+  const int n128 = (a.N + 127) / 128;
+  // Few tiles of a long sum: more waves of a tile share its K-tiles. (3 rows of 4 experts, 4096 x 2048:
+  // one set of waves 32 us, 2 20, 4 18; 16 rows of 16, 4096 x 4096: 82, 82, 88; 25 rows of each of 4,
+  // 2048 x 1024: 16.9, 12.5, 12.7.)
+  const bool long_sum = a.K >= 16 * (DT == kF32 ? 32 : 64);
+  const double few = row_tiles(a, avg <= 16 ? 16 : 32) * n128;
+  if (avg <= 16) {
+    if (long_sum && few <= 128) return launch<DT, false, B_KC, 16, 128, 1, 1, 4>(a, buf, s);
+    if (long_sum && few <= 256) return launch<DT, false, B_KC, 16, 128, 1, 1, 2>(a, buf, s);
+    return launch<DT, false, B_KC, 16, 128, 1, 1>(a, buf, s);
+  }
   if constexpr (DT == kF32) {
     // an MFMA of 4 k takes as long as one of 32 in 16 bits: small tiles lose nothing to
     // loads, and pad groups and widths less (8 experts of 512 rows, 2048 x 2048: 32 x 64
@@ -376,8 +410,11 @@ hipError_t launch_rows(const GroupArgs& a, bool buf, bool large, hipStream_t s) 
     if (avg <= 256) return launch<DT, false, B_KC, 32, 64, 2, 2>(a, buf, s);
     return launch<DT, false, B_KC, 64, 64, 2, 2>(a, buf, s);
   } else {
-    if (avg <= 32) return launch<DT, false, B_KC, 32, 128, 1, 1>(a, buf, s);
-    const int n256 = (a.N + 255) / 256, n128 = (a.N + 127) / 128;
+    if (avg <= 32) {
+      if (long_sum && few <= 256) return launch<DT, false, B_KC, 32, 128, 1, 1, 2>(a, buf, s);
+      return launch<DT, false, B_KC, 32, 128, 1, 1>(a, buf, s);
+    }
+    const int n256 = (a.N + 255) / 256;
     const double t64 = tile_time(row_tiles(a, 64) * n128, 0.6, 1.8, 3);
     const double t128 = tile_time(row_tiles(a, 128) * n128, 0.87, 1.83, 2);
     if (large && large_time(row_tiles(a, 256) * n256) <= (t64 < t128 ? t64 : t128))

@@ -284,3 +284,40 @@ def test_an_expert_layer_trained_and_served():
         ref = torch.nn.functional.silu(a) @ plain[1][who[t]]
         # bf16 roundings: of h, of silu(h) (its slope is below 1.1) and of the result
         assert ((out[0].double() - ref).norm() / ref.norm()).item() < 3.3 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("colmajor", [False, True], ids=["row", "col"])
+@pytest.mark.parametrize("sizes,K,N", [
+    ([1, 0, 2], 1500, 264),      # few tiles of a long sum: four sets of waves share a tile's k
+    ([9] * 14, 1096, 1920),      # two sets
+    ([25, 30, 0, 20], 2056, 520),
+    ([33, 40, 64, 50], 1024, 384),
+    ([100, 128, 90], 520, 768),
+])
+def test_long_sums(dtype, colmajor, sizes, K, N):
+    x, w = _data(sum(sizes) + 1, K, N, len(sizes), DT[dtype], colmajor)
+    ends = _ends(sizes)
+    _close(ops.grouped_matmul(x, w, ends), _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
+
+
+@pytest.mark.parametrize("sizes", [[200, 0, 1, 63, 64, 65, 129, 300], [0, 0, 700, 0], [5] * 8])
+def test_large_tiles_of_ragged_sums(sizes):
+    """Weight gradients whose sums are shorter than the large tiles' four K-tiles, end inside one, or
+    are empty, beside each other in one stream."""
+    x, _ = _data(sum(sizes), 520, 1, 1, torch.bfloat16)
+    dy, _ = _data(sum(sizes), 776, 1, 1, torch.bfloat16, seed=5)
+    ends = _ends(sizes)
+    _close(ops.grouped_weight_grad(x, dy, ends), _reduce_exact(x, dy, ends),
+           _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
+
+
+def test_many_experts_on_large_tiles():
+    """More experts than one wave scans, on the large tiles' stream, several tiles a CU."""
+    sizes = [(i * 37) % 200 + 30 for i in range(150)]
+    x, w = _data(sum(sizes), 200, 512, 150, torch.float16)
+    ends = _ends(sizes)
+    _close(ops.grouped_matmul(x, w, ends), _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), 200)
+    dy, _ = _data(sum(sizes), 264, 1, 1, torch.float16, seed=5)
+    _close(ops.grouped_weight_grad(x, dy, ends), _reduce_exact(x, dy, ends),
+           _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
