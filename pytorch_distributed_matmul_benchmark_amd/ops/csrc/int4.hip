@@ -38,6 +38,7 @@ struct Args : GroupArgs {
   const void* scale;
   const unsigned char* zero;
   int groups;   // K / G
+  long long scales;  // E N groups
   unsigned chunk_g;  // G > 128: ceil(2^32 / (G / 128)), else 0
 };
 
@@ -148,38 +149,54 @@ struct ScaleBlock {
   static constexpr int CHUNKS = KB, PIECES = COLS * NG / 8, CH = (PIECES + THREADS - 1) / THREADS;
   u32x4 s[CH];
   u32x2 z[CH];
-  // groups from g0 of columns from n0 (of expert e's `first`); what is not there is zero
+  int back[CH];  // groups the load was moved back by, not to pass the array's end
+  // groups from g0 of columns from n0 (of expert e's `first`); what is not there is stored as zero
   __device__ __forceinline__ void load(const Args& a, long long first, int n0, int g0, int tid) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int at = tid + i * THREADS, col = at / (NG / 8), gr = g0 + at % (NG / 8) * 8;
       const long long off = (first + min(n0 + col, a.N - 1)) * a.groups + gr;
-      const unsigned short* sp = (const unsigned short*)a.scale + off;
-      const unsigned char* zp = a.zero + off;
-      s[i] = u32x4{0u, 0u, 0u, 0u};
-      z[i] = u32x2{0u, 0u};
-      if (gr + 8 <= a.groups) {
-        __builtin_memcpy(&s[i], sp, 16);
-        if constexpr (ZERO) __builtin_memcpy(&z[i], zp, 8);
-      } else {
+      if (a.scales < 8) {  // (uniform)
+        s[i] = u32x4{0u, 0u, 0u, 0u};
+        z[i] = u32x2{0u, 0u};
+        back[i] = 0;
 #pragma unroll
         for (int t = 0; t < 7; ++t)
-          if (gr + t < a.groups) {
-            s[i][t >> 1] |= (unsigned)sp[t] << (16 * (t & 1));
-            if constexpr (ZERO) z[i][t >> 2] |= (unsigned)zp[t] << (8 * (t & 3));
+          if (off + t < a.scales) {
+            s[i][t >> 1] |= (unsigned)((const unsigned short*)a.scale)[off + t] << (16 * (t & 1));
+            if constexpr (ZERO) z[i][t >> 2] |= (unsigned)a.zero[off + t] << (8 * (t & 3));
           }
+        continue;
       }
+      // (no branch around these loads: each would wait for its own)
+      const long long at8 = off < a.scales - 8 ? off : a.scales - 8;
+      __builtin_memcpy(&s[i], (const unsigned short*)a.scale + at8, 16);
+      if constexpr (ZERO) __builtin_memcpy(&z[i], a.zero + at8, 8);
+      back[i] = (int)(off - at8);
     }
   }
-  __device__ __forceinline__ void store(char* lds, int tid) const {
+  __device__ __forceinline__ void store(const Args& a, char* lds, int g0, int tid) const {
+    typedef unsigned long long u64;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int at = tid + i * THREADS, col = at / (NG / 8), gr = at % (NG / 8) * 8;
+      u64 lo = (u64)s[i][1] << 32 | s[i][0], hi = (u64)s[i][3] << 32 | s[i][2], zz = 0;
+      if constexpr (ZERO) zz = (u64)z[i].y << 32 | z[i].x;
+      const int left = a.groups - g0 - gr;  // groups from here to the column's last
+      if (left < 8) {
+        const int b = min(back[i], 8);
+        lo = b >= 8 ? 0 : b >= 4 ? hi >> (16 * (b - 4)) : b ? lo >> (16 * b) | hi << (64 - 16 * b) : lo;
+        hi = b >= 4 ? 0 : hi >> (16 * b);
+        zz = b >= 8 ? 0 : zz >> (8 * b);
+        if (left < 4) lo = left <= 0 ? 0 : lo & ((1ull << (16 * left)) - 1);
+        hi = left <= 4 ? 0 : hi & ((1ull << (16 * (left - 4))) - 1);
+        zz = left <= 0 ? 0 : zz & ((1ull << (8 * left)) - 1);
+      }
       if (PIECES % THREADS == 0 || at < PIECES) {
         char* p = lds + col * SP + 2 * gr;
-        *(lds_u32x2*)p = u32x2{s[i][0], s[i][1]};
-        *(lds_u32x2*)(p + 8) = u32x2{s[i][2], s[i][3]};
-        if constexpr (ZERO) *(lds_u32x2*)(lds + COLS * SP + col * ZP + gr) = z[i];
+        *(lds_u32x2*)p = u32x2{(unsigned)lo, (unsigned)(lo >> 32)};
+        *(lds_u32x2*)(p + 8) = u32x2{(unsigned)hi, (unsigned)(hi >> 32)};
+        if constexpr (ZERO) *(lds_u32x2*)(lds + COLS * SP + col * ZP + gr) = u32x2{(unsigned)zz, (unsigned)(zz >> 32)};
       }
     }
   }
@@ -327,7 +344,7 @@ __device__ __forceinline__ void few_sums(const Args& a, const RowTile& r, int n0
 #pragma unroll
       for (int d = 0; d < D; ++d) load(st[d], c + d);
       if (k0 > 0) __syncthreads();  // the block before is used up
-      sb.store(sl, tid);
+      sb.store(a, sl, g0, tid);
       __syncthreads();
       auto mul = [&](Step<NB, RX>& b, int c) {
         const int at = SG > 1 ? (c - k0) * SG : group_of(a, c) - g0;
@@ -473,7 +490,9 @@ __global__ void __launch_bounds__(256 * KW) gemm_int4_rows(Args a) {
           __builtin_bit_cast(u32x4, permute_row(xs[i]));
     }
   };
+  SB sb;
   if (np > 0) {
+    sb.load(a, first, tn * BN, 0, tid);
     load(0);
     ready(0);
     load(1);
@@ -482,10 +501,11 @@ __global__ void __launch_bounds__(256 * KW) gemm_int4_rows(Args a) {
   for (int step = 0; step < np; ++step) {
     if (step % (KB / KW) == 0) {  // the scales of the next KB chunks
       g0 = SG > 1 ? KW * step * SG : group_of(a, KW * step);
-      SB sb;
-      sb.load(a, first, tn * BN, g0, tid);
-      if (step) __syncthreads();  // those before are used up
-      sb.store(sl, tid);
+      if (step) {
+        sb.load(a, first, tn * BN, g0, tid);
+        __syncthreads();  // those before are used up
+      }
+      sb.store(a, sl, g0, tid);
     }
     // this step's rows are written, and the other buffer's readers are done (loads stay in flight)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -591,13 +611,20 @@ hipError_t launch_rows(Args a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Row tiles of bm rows, as many as the rows fill on average where groups share them.
+inline long long tiles_about(const Args& a, int bm) {
+  if (!a.ends) return (a.T + bm - 1) / bm;
+  const long long full = (a.T + (long long)a.E * bm / 2) / bm, groups = a.T < a.E ? a.T : a.E;
+  return full > groups ? full : groups;
+}
+
 template <int DT, int SG, int RX, bool ZERO>
 hipError_t pick_few(const Args& a, hipStream_t s) {
   // Waves a tile: enough to fill the CUs where there are few tiles (1 x 4096 x 4096: 8
   // waves 4.5 us, 4 5.2), no more where there are many — the chip starts about 3.5
   // waves a ns (16 x 4096 x 11007: 4 waves 11.7 us, 2 15.0; 64 experts 2048 x 2048 of
   // 64 rows, 32 columns a tile: 2 waves 27 us, 4 29, 8 43; 16 columns and 2 waves 30).
-  const long long tiles = (long long)(a.ends ? (a.T < a.E ? a.T : a.E) : 1) * ((a.N + 15) / 16);
+  const long long tiles = tiles_about(a, 16) * ((a.N + 15) / 16);
   if (tiles >= 4096) return launch_few<DT, 2, SG, RX, ZERO, 2>(a, s);
   if (tiles > 512) return launch_few<DT, 1, SG, RX, ZERO, 4>(a, s);
   return launch_few<DT, 1, SG, RX, ZERO, 8>(a, s);
@@ -605,14 +632,29 @@ hipError_t pick_few(const Args& a, hipStream_t s) {
 
 template <int DT, int SG, bool ZERO>
 hipError_t pick(const Args& a, hipStream_t s) {
-  const int avg = (a.T + a.E - 1) / a.E;
   if (a.T <= 4) return pick_few<DT, SG, 1, ZERO>(a, s);
-  if (avg <= 16) return pick_few<DT, SG, 4, ZERO>(a, s);
-  // (100 x 4096 x 8192, groups of 64: 64 rows in 4 parts of k 21.6 us, 2 parts 24.0; 32 rows 26;
-  // 512 rows: 128 columns 67 us, 64 72. 32 rows: 4 parts 14.2, 2 15.7.)
-  if (avg <= 32) return launch_rows<DT, 2, 1, SG, ZERO, 4>(a, s);
-  if (blocks_of(a, 64, 128) >= 512) return launch_rows<DT, 4, 2, SG, ZERO, 2>(a, s);
-  return launch_rows<DT, 4, 1, SG, ZERO, 4>(a, s);
+  if ((a.T + a.E - 1) / a.E <= 16) return pick_few<DT, SG, 4, ZERO>(a, s);
+  // More rows than 16: the least of the times of the grids, in us. The tall tiles read
+  // and widen the weights fewer times, but a workgroup of theirs fills a CU: a round of
+  // 256 costs what one does (us a step of 512 k: 16 rows 1.0, 32 1.35, 64 1.95; of 64
+  // rows x 128 columns a step of 256 k: 1.9). Tiles of 16 x 16 cost a step's latency a
+  // wave, or the sum of their work. Measured, us: 25 x 1024 x 5632: 16 x 16 6.4, 32
+  // rows 14.5; 33 x 448 x 5216 7.0, 32 rows 17, 64 23; 47 x 4480 x 10176 29, 27, 35;
+  // 64 x 8192 x 4096 22, 15.5, 20; 64 x 16384 x 4096 35, 27, 21.5; 512 x 4096 x 4096: 64
+  // rows 41, with 128 columns 35.
+  const int chunks = (a.K + 127) / 128, steps = (chunks + 3) / 4;
+  auto rounds = [&](int bm, int bn) { return (int)((tiles_about(a, bm) * ((a.N + bn - 1) / bn) + 255) / 256); };
+  const double type = DT == kF16 ? 0.8 : 1.0;
+  const double work = tiles_about(a, 16) * ((a.N + 15) / 16) * (double)chunks;
+  const double few = work * 0.00035 > chunks * 0.08 ? work * 0.00035 : chunks * 0.08;
+  const double t16 = 0.5 + type * 1.0 * rounds(16, 64) * steps, t32 = 0.5 + type * 1.35 * rounds(32, 64) * steps,
+               t64 = 0.5 + type * 1.95 * rounds(64, 64) * steps,
+               wide = 0.5 + type * 1.9 * rounds(64, 128) * ((chunks + 1) / 2);
+  const double lo = t16 < t32 ? t16 : t32, hi = t64 < wide ? t64 : wide;
+  if (few <= lo && few <= hi) return pick_few<DT, SG, 4, ZERO>(a, s);
+  if (lo <= hi)
+    return t16 < t32 ? launch_rows<DT, 1, 1, SG, ZERO, 4>(a, s) : launch_rows<DT, 2, 1, SG, ZERO, 4>(a, s);
+  return t64 <= wide ? launch_rows<DT, 4, 1, SG, ZERO, 4>(a, s) : launch_rows<DT, 4, 2, SG, ZERO, 2>(a, s);
 }
 
 template <int DT, bool ZERO>
@@ -649,6 +691,7 @@ hipError_t int4_gemm(const Int4Problem& p, hipStream_t stream) {
   a.scale = p.scale;
   a.zero = (const unsigned char*)p.zero;
   a.groups = p.K / p.G;
+  a.scales = (long long)p.E * p.N * a.groups;
   a.chunk_g = p.G > 128 ? (unsigned)(((1ll << 32) + p.G / 128 - 1) / (p.G / 128)) : 0u;
   if (p.dtype == kBF16) return kint4::pick_zero<kBF16>(a, p.G, stream);
   if (p.dtype == kF16) return kint4::pick_zero<kF16>(a, p.G, stream);

@@ -52,9 +52,20 @@ def test_one_weight(dtype, zero, M, N, K, G):
     _close(y, x, *_values(q, s, z), K // G)
 
 
+# enough columns that the rows are taken 16, 32, 64 and 64 (of 128 columns) a tile
+@pytest.mark.parametrize("M,N,K", [(33, 5400, 2048), (64, 8001, 640), (130, 5000, 1152), (500, 4090, 768)])
+@pytest.mark.parametrize("G,zero", [(32, True), (64, False), (64, True), (128, True), (128, False)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_many_columns(dtype, G, zero, M, N, K):
+    q, s, z = _weight((), N, K, G, DT[dtype], zero)
+    x = torch.randn(M, K, device="cuda").to(DT[dtype])
+    _close(ops.int4_matmul(x, q, s, z), x, *_values(q, s, z), K // G)
+
+
 @pytest.mark.parametrize("sizes,behind,N,K,G", [
     ([1], 0, 40, 64, 32), ([0, 3, 1, 0], 2, 136, 256, 64), ([1] * 66, 0, 48, 128, 128),
-    ([17, 0, 40, 2], 0, 100, 416, 32), ([100, 64, 1], 5, 272, 768, 256)])
+    ([17, 0, 40, 2], 0, 100, 416, 32), ([100, 64, 1], 5, 272, 768, 256),
+    ([100, 64, 1, 70], 3, 4100, 416, 32), ([30, 0, 32, 20], 70, 5000, 1024, 64)])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_expert_weights(dtype, sizes, behind, N, K, G):
     dt, T = DT[dtype], sum(sizes) + behind
