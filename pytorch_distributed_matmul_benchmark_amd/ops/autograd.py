@@ -71,5 +71,7 @@ def native_grouped_matmul(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) 
     w[e]^T`` on the same kernel (the transposed weights are read in place) and
     ``dw[e] = x_e^T @ dy_e`` (``grouped.grouped_weight_grad``). Rows behind the last
     expert's, and experts without rows, get zero gradients. ``ends`` must not
-    change between the forward and the backward pass."""
-    return _NativeGroupedMatmul.apply(x, w, ends)
+    change between the forward and the backward pass. Under a stream capture a leaf
+    whose graph from the default stream is still alive is refused."""
+    res = grouped._native_call("grouped_node", x, w, ends)
+    return _NativeGroupedMatmul.apply(x, w, ends) if res is None else res

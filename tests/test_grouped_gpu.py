@@ -321,3 +321,75 @@ def test_many_experts_on_large_tiles():
     dy, _ = _data(sum(sizes), 264, 1, 1, torch.float16, seed=5)
     _close(ops.grouped_weight_grad(x, dy, ends), _reduce_exact(x, dy, ends),
            _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
+
+
+def test_no_second_derivative():
+    x = torch.randn(5, 16, device="cuda", requires_grad=True)
+    w = torch.randn(2, 16, 8, device="cuda", requires_grad=True)
+    ends = torch.tensor([2, 5], device="cuda")
+    y = ops.native_grouped_matmul(x, w, ends)
+    want = torch.autograd.grad(y.square().sum(), (x, w), retain_graph=True)
+    got = torch.autograd.grad(y.square().sum(), (x, w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError, match="differentiate|derivative"):
+        torch.autograd.grad(got[0].sum() + got[1].sum(), (x, w))
+
+
+@pytest.mark.parametrize("grads", ["x", "w", "both", "neither"])
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradients_of_what_asks_for_them(grads, strided):
+    """Gradients go to the leaves that ask for them, also where an operand is copied first."""
+    x = torch.randn(7, 24, device="cuda").bfloat16()
+    w = torch.randn(3, 24, 40, device="cuda").bfloat16()
+    if strided:
+        x, w = torch.stack((x, x), -1)[..., 0], torch.stack((w, w), -1)[..., 0]
+    x.requires_grad_(grads in ("x", "both"))
+    w.requires_grad_(grads in ("w", "both"))
+    ends = torch.tensor([3, 3, 6], device="cuda")
+    y = ops.native_grouped_matmul(x, w, ends)
+    with torch.no_grad():
+        assert torch.equal(y, ops.grouped_matmul(x, w, ends))
+    assert y.requires_grad == (grads != "neither")
+    if grads == "neither":
+        return
+    y.sum().backward()  # (an expanded gradient)
+    dy = torch.ones_like(y)
+    with torch.no_grad():
+        if x.requires_grad:
+            assert torch.equal(x.grad, ops.grouped_matmul(dy, w.transpose(1, 2), ends))
+        if w.requires_grad:
+            assert torch.equal(w.grad, ops.grouped_weight_grad(x, dy, ends))
+    assert (x.grad is not None) == x.requires_grad and (w.grad is not None) == w.requires_grad
+
+
+def test_an_operand_changed_before_the_backward_pass_is_refused():
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    w = torch.randn(2, 16, 16, device="cuda", requires_grad=True)
+    ends = torch.tensor([2, 4], device="cuda")
+    y = ops.native_grouped_matmul(x, w, ends)
+    ends.add_(0)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_capture_beside_a_living_eager_graph_is_refused(strided):
+    x = torch.randn(4, 16, device="cuda")
+    x = (torch.stack((x, x), -1)[..., 0] if strided else x).requires_grad_()
+    w = torch.randn(2, 16, 16, device="cuda", requires_grad=True)
+    ends = torch.tensor([2, 4], device="cuda")
+    alive = ops.native_grouped_matmul(x, w, ends)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.native_grouped_matmul(x, w, ends)
+    dx, dw = torch.autograd.grad(alive.sum(), (x, w))
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.native_grouped_matmul(x, w, ends)
+    for _ in range(3):
+        y.detach().zero_()
+        graph.replay()
+        with torch.no_grad():
+            assert torch.equal(y, ops.grouped_matmul(x, w, ends))
