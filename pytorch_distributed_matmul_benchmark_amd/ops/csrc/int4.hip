@@ -156,22 +156,27 @@ struct ScaleBlock {
     for (int i = 0; i < CH; ++i) {
       const int at = tid + i * THREADS, col = at / (NG / 8), gr = g0 + at % (NG / 8) * 8;
       const long long off = (first + min(n0 + col, a.N - 1)) * a.groups + gr;
-      if (a.scales < 8) {  // (uniform)
-        s[i] = u32x4{0u, 0u, 0u, 0u};
-        z[i] = u32x2{0u, 0u};
-        back[i] = 0;
-#pragma unroll
-        for (int t = 0; t < 7; ++t)
-          if (off + t < a.scales) {
-            s[i][t >> 1] |= (unsigned)((const unsigned short*)a.scale)[off + t] << (16 * (t & 1));
-            if constexpr (ZERO) z[i][t >> 2] |= (unsigned)a.zero[off + t] << (8 * (t & 3));
-          }
-        continue;
-      }
       // (no branch around these loads: each would wait for its own)
-      const long long at8 = off < a.scales - 8 ? off : a.scales - 8;
-      __builtin_memcpy(&s[i], (const unsigned short*)a.scale + at8, 16);
-      if constexpr (ZERO) __builtin_memcpy(&z[i], a.zero + at8, 8);
+      const long long at8 = off < a.scales - 8 ? off : a.scales < 8 ? 0 : a.scales - 8;
+      const unsigned short* sp = (const unsigned short*)a.scale + at8;
+      const unsigned char* zp = a.zero + at8;
+      u32x4 v;
+      u32x2 w = {0u, 0u};
+      if (a.scales >= 8) {
+        __builtin_memcpy(&v, sp, 16);
+        if constexpr (ZERO) __builtin_memcpy(&w, zp, 8);
+      } else {  // (fewer in all: each by itself, the last one again past the end)
+        const int n = (int)a.scales - 1;
+        auto pair = [&](int t) { return (unsigned)sp[min(t, n)] | (unsigned)sp[min(t + 1, n)] << 16; };
+        v = u32x4{pair(0), pair(2), pair(4), pair(6)};
+        auto four = [&](int t) {
+          return (unsigned)zp[min(t, n)] | (unsigned)zp[min(t + 1, n)] << 8 | (unsigned)zp[min(t + 2, n)] << 16 |
+                 (unsigned)zp[min(t + 3, n)] << 24;
+        };
+        if constexpr (ZERO) w = u32x2{four(0), four(4)};
+      }
+      s[i] = v;
+      z[i] = w;
       back[i] = (int)(off - at8);
     }
   }
