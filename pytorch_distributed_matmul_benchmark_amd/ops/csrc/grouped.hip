@@ -22,8 +22,9 @@
 // of 4 bytes come as 16-byte buffer loads whose descriptor ends with the tile's last
 // row (KC) or k (KS), moved along k, so that what is not there reads as zero with no
 // branch (a branch around a load makes hipcc wait for later loads too); only a row
-// that ends inside 16 bytes is masked, in its last K-tile. Others are read with any
-// alignment, by the element at the edges.
+// that ends inside 16 bytes is masked, in its last K-tile. 16-bit operands of odd
+// strides are read as the five aligned dwords around a chunk and shifted on their way
+// to LDS. Strides past 8 MB are read by the element at the edges.
 #include "api.h"
 #include "grouped.h"
 
@@ -33,6 +34,7 @@ namespace pdmb {
 namespace kgrp {
 
 constexpr int NT = 256;
+enum Loads { kAny, kDwords, kOdd };  // how the operands are read (above)
 
 template <int DT>
 constexpr int esize() { return DT == kF32 ? 4 : 2; }
@@ -70,7 +72,7 @@ __device__ __forceinline__ u32x4 keep(u32x4 v, int avail) {
 }
 
 // One operand tile of R rows (or columns) x one K-tile.
-template <int DT, bool KC, int R, bool BUF>
+template <int DT, bool KC, int R, int BUF>
 struct Tile {
   static constexpr int ES = esize<DT>(), EPC = 16 / ES, BK = 128 / ES;
   static constexpr int BYTES = R * 128;
@@ -83,9 +85,10 @@ struct Tile {
   long long ld;    // leading stride
   int rows, ks;    // what there is of it
   int first;       // lane's offset of chunk 0 in bytes (BUF)
+  int odd;         // kOdd: bytes of p past a dword
 
   __device__ __forceinline__ Tile(const char* p_, long long ld_, int rows_, int ks_, int tid)
-      : p(p_), ld(ld_), rows(rows_ < R ? rows_ : R), ks(ks_) {
+      : p(p_), ld(ld_), rows(rows_ < R ? rows_ : R), ks(ks_), odd(BUF == kOdd ? (int)((uintptr_t)p_ & 2) : 0) {
     first = KC ? (tid >> 3) * (int)(ld * ES) + (tid & 7) * 16 : tid / CPK * (int)(ld * ES) + tid % CPK * 16;
   }
   // LDS offset of chunk idx
@@ -104,18 +107,28 @@ struct Tile {
     }
   }
   // Global loads of the K-tile at k0 (past ks: zeros).
-  __device__ __forceinline__ void load(u32x4 (&v)[CH], int k0, int tid) const {
-    if constexpr (BUF) {
+  // kOdd: the dwords around a chunk, v and then x; store() shifts them.
+  __device__ __forceinline__ void load(u32x4 (&v)[CH], unsigned (&x)[CH], int k0, int tid) const {
+    if constexpr (BUF != kAny) {
       // from here to the last element of the tile's last row (KC) or k (KS)
       const long long from = KC ? (long long)k0 * ES : (long long)k0 * ld * ES;
       const long long bytes = (KC ? (long long)(rows - 1) * ld + ks : (long long)(ks - 1) * ld + rows) * ES - from;
-      const u32x4 d = make_rsrc(p + from, (bytes + 3) & ~3ll);  // (a dword that the end cuts counts as inside)
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((char*)(p + from), 0, (int)d.z, 0x00020000);
+      const char* base = p + from - odd;
+      const u32x4 d = make_rsrc(base, (bytes + odd + 3) & ~3ll);  // (a dword that the end cuts counts as inside)
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((char*)base, 0, (int)d.z, 0x00020000);
       const int step = (int)(ld * ES) * (KC ? 32 : NT / CPK);  // bytes between a lane's chunks
       const int out = KC && (tid & 7) * EPC >= ks - k0 ? (int)0x80000000 : 0;  // k past the end of a row
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (first + i * step) | out, 0, 0));
+      for (int i = 0; i < CH; ++i) {
+        int o = first + i * step;
+        if constexpr (BUF == kOdd) {
+          o = (o + odd) & ~3;
+          // (the dword that holds the last element may hold the k after it too)
+          if (!KC && k0 + (tid + i * NT) / CPK >= ks) o = (int)0x80000000;
+        }
+        v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o | out, 0, 0));
+        if constexpr (BUF == kOdd) x[i] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rs, (o | out) + 16, 0, 0);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
@@ -130,8 +143,17 @@ struct Tile {
       }
     }
   }
-  __device__ __forceinline__ void store(char* lds, u32x4 (&v)[CH], int k0, int tid) const {
-    if (BUF && KC && ks % EPC && k0 + BK > ks) {  // the row ends inside 16 bytes: what follows it is not zero
+  __device__ __forceinline__ void store(char* lds, u32x4 (&v)[CH], const unsigned (&x)[CH], int k0, int tid) const {
+    if constexpr (BUF == kOdd) {
+      const int step = (int)(ld * ES) * (KC ? 32 : NT / CPK);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int by = ((first + odd + i * step) & 2) * 8;
+        v[i] = u32x4{__builtin_amdgcn_alignbit(v[i][1], v[i][0], by), __builtin_amdgcn_alignbit(v[i][2], v[i][1], by),
+                     __builtin_amdgcn_alignbit(v[i][3], v[i][2], by), __builtin_amdgcn_alignbit(x[i], v[i][3], by)};
+      }
+    }
+    if (BUF != kAny && KC && ks % EPC && k0 + BK > ks) {  // the row ends inside 16 bytes: what follows it is not zero
 #pragma unroll
       for (int i = 0; i < CH; ++i) v[i] = keep<DT>(v[i], ks - k0 - (tid & 7) * EPC);
     }
@@ -175,32 +197,9 @@ __device__ __forceinline__ void mma(f32x4& acc, const u32x4& b, const u32x4& a) 
   }
 }
 
-// Four columns of one row, `left` of them inside C; whole: 4 elements at once where they all are.
-template <int DT>
-__device__ __forceinline__ void store4(char* p, const f32x4& v, int left, bool whole) {
-  if constexpr (DT == kF32) {
-    if (whole && left >= 4) {
-      *(f32x4*)p = v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) ((float*)p)[j] = v[j];
-    }
-  } else {
-    const u32x2 w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-    if (whole && left >= 4) {
-      *(u32x2*)p = w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) ((unsigned short*)p)[j] = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
-    }
-  }
-}
-
 // RED: `reduce` (A and B are both KS). BM x BN tile, WR x 4 / WR waves; KW > 1: KW such
 // sets of waves take every KW-th K-tile, and their sums meet in LDS, added in order.
-template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, bool BUF, int KW>
+template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, int BUF, int KW>
 __global__ void __launch_bounds__(NT * KW) gemm_grouped(GroupArgs a) {
   constexpr int ES = esize<DT>();
   using TA = Tile<DT, !RED, BM, BUF>;
@@ -255,10 +254,11 @@ __global__ void __launch_bounds__(NT * KW) gemm_grouped(GroupArgs a) {
     const TA ta(Ap, a.lda, rows, ks, tid);
     const TB tb(Bp, a.ldb, cols, ks, tid);
     u32x4 va[PF][TA::CH], vb[PF][TB::CH];
+    unsigned xa[PF][TA::CH], xb[PF][TB::CH];
 #pragma unroll
     for (int d = 0; d < PF; ++d) {
-      ta.load(va[d], (d * KW + kw) * BK, tid);
-      tb.load(vb[d], (d * KW + kw) * BK, tid);
+      ta.load(va[d], xa[d], (d * KW + kw) * BK, tid);
+      tb.load(vb[d], xb[d], (d * KW + kw) * BK, tid);
     }
     for (int t0 = 0; t0 * KW < nk; t0 += PF) {
 #pragma unroll
@@ -266,10 +266,10 @@ __global__ void __launch_bounds__(NT * KW) gemm_grouped(GroupArgs a) {
         const int t = t0 + d;  // K-tile t KW + kw (past the end: zeros)
         if (PF > 1 && t * KW >= nk) break;
         char* st = smem + (kw * 2 + (t & 1)) * STAGE;
-        ta.store(st, va[d], (t * KW + kw) * BK, tid);
-        tb.store(st + TA::BYTES, vb[d], (t * KW + kw) * BK, tid);
-        ta.load(va[d], ((t + PF) * KW + kw) * BK, tid);
-        tb.load(vb[d], ((t + PF) * KW + kw) * BK, tid);
+        ta.store(st, va[d], xa[d], (t * KW + kw) * BK, tid);
+        tb.store(st + TA::BYTES, vb[d], xb[d], (t * KW + kw) * BK, tid);
+        ta.load(va[d], xa[d], ((t + PF) * KW + kw) * BK, tid);
+        tb.load(vb[d], xb[d], ((t + PF) * KW + kw) * BK, tid);
         // this stage is written; the other one's readers are done (LDS only: loads stay in flight)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
@@ -312,57 +312,72 @@ __global__ void __launch_bounds__(NT * KW) gemm_grouped(GroupArgs a) {
   // from the accumulators, a row's 32 bytes at a time, a weight gradient of 48 experts
   // of 167 rows, 2048 x 1024, takes 113 us instead of 80.
   constexpr int ROWB = NB * 16 * ES, PITCH = ROWB + 16, LPR = ROWB / 16, RPI = 64 / LPR;
-  static_assert(4 * 16 * PITCH <= 2 * STAGE && 16 % RPI == 0, "epilogue rows");
-  if ((uintptr_t)a.C % 16 == 0 && a.ldc * ES % 16 == 0 && a.sC * ES % 16 == 0 && a.N * ES % 16 == 0) {
-    typedef __attribute__((address_space(3))) char lds_char;
-    lds_char* eb = (lds_char*)(lds_void*)(smem + w * 16 * PITCH);
-    if constexpr (KW == 1) __syncthreads();  // the last K-tile is read
-    const int rl = lane / LPR, cb = lane % LPR * 16;
-    const bool in = wc * ROWB + cb < cols * ES;
+  static_assert(4 * 16 * PITCH <= 2 * STAGE && 16 % RPI == 0 && 64 % (ROWB / 4) == 0, "epilogue rows");
+  typedef __attribute__((address_space(3))) char lds_char;
+  lds_char* eb = (lds_char*)(lds_void*)(smem + w * 16 * PITCH);
+  const bool pieces = (uintptr_t)a.C % 16 == 0 && a.ldc * ES % 16 == 0 && a.sC * ES % 16 == 0 && a.N * ES % 16 == 0;
+  const int col0 = wc * (BN / WC);
+  if constexpr (KW == 1) __syncthreads();  // the last K-tile is read
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
+  for (int i = 0; i < MB; ++i) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        lds_char* p = eb + l16 * PITCH + (j * 16 + 4 * g) * ES;
-        if constexpr (DT == kF32) *(__attribute__((address_space(3))) f32x4*)p = acc[i][j];
-        else *(lds_u32x2*)p = u32x2{pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3])};
-      }
+    for (int j = 0; j < NB; ++j) {
+      lds_char* p = eb + l16 * PITCH + (j * 16 + 4 * g) * ES;
+      if constexpr (DT == kF32) *(__attribute__((address_space(3))) f32x4*)p = acc[i][j];
+      else *(lds_u32x2*)p = u32x2{pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3])};
+    }
+    const int row0 = wr * (BM / WR) + i * 16;
+    if (pieces) {
+      const int rl = lane / LPR, cb = lane % LPR * 16;
+      const bool in = col0 * ES + cb < cols * ES;
 #pragma unroll
       for (int r = 0; r < 16 / RPI; ++r) {
         const u32x4 x = *(lds_u32x4_t*)(eb + (r * RPI + rl) * PITCH + cb);
-        const int row = wr * (BM / WR) + i * 16 + r * RPI + rl;
-        if (in && row < rows) __builtin_nontemporal_store(x, (u32x4*)(Cp + row * a.ldc * ES + wc * ROWB + cb));
+        const int row = row0 + r * RPI + rl;
+        if (in && row < rows) __builtin_nontemporal_store(x, (u32x4*)(Cp + row * a.ldc * ES + col0 * ES + cb));
       }
-    }
-    return;
-  }
-  const bool whole = (uintptr_t)a.C % (4 * ES) == 0 && a.ldc % 4 == 0 && a.sC % 4 == 0;
+    } else {
+      // Rows at any element: whole dwords of C, and the elements at a row's ends by themselves.
+      constexpr int DPR = ROWB / 4, RPD = 64 / DPR;  // dwords a row, rows at once
+      const int rl = lane / DPR, d = lane % DPR;
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int r = wr * (BM / WR) + i * 16 + l16;
-    if (r < rows) {
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const int c = wc * (BN / WC) + j * 16 + 4 * g;
-        store4<DT>(Cp + ((long long)r * a.ldc + c) * ES, acc[i][j], cols - c, whole);
+      for (int r = 0; r < 16 / RPD; ++r) {
+        const int rr = r * RPD + rl, row = row0 + rr;
+        if (row < rows) {
+          char* q = Cp + (row * a.ldc + col0) * ES;
+          if constexpr (ES == 4) {
+            const unsigned x = *(const __attribute__((address_space(3))) unsigned*)(eb + rr * PITCH + 4 * d);
+            if (col0 + d < cols) *(unsigned*)(q + 4 * d) = x;
+          } else {
+            typedef const __attribute__((address_space(3))) unsigned short lds_u16;
+            const int off = (int)((uintptr_t)q >> 1) & 1, c = 2 * d + off;  // this lane's two columns
+            const lds_u16* p = (const lds_u16*)(eb + rr * PITCH);
+            const unsigned lo = p[c], hi = c + 1 < ROWB / 2 ? p[c + 1] : 0u;
+            const int left = min(cols - col0, ROWB / 2) - c;
+            if (left > 1) *(unsigned*)(q + 2 * c) = lo | hi << 16;
+            if (left == 1) *(unsigned short*)(q + 2 * c) = (unsigned short)lo;
+            if (off && d == 0 && cols > col0) *(unsigned short*)q = p[0];
+          }
+        }
       }
     }
   }
 }
 
 template <int DT, bool RED, bool B_KC, int BM, int BN, int WR, int PF, int KW = 1>
-hipError_t launch(GroupArgs a, bool buf, hipStream_t s) {
+hipError_t launch(GroupArgs a, int buf, hipStream_t s) {
   a.tiles_m = (a.M + BM - 1) / BM;
   a.tiles_n = (a.N + BN - 1) / BN;
   const long long blocks = RED ? (long long)a.E * a.tiles_m * a.tiles_n
                                : (row_tiles_bound(a.T, a.E, BM, a.zero_tail) * a.tiles_n + 7) / 8 * 8;
   if (blocks > (1ll << 30)) return hipErrorInvalidValue;
-  if (buf)
-    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, PF, true, KW>), dim3((unsigned)blocks), dim3(NT * KW), 0,
-                       s, a);
+  const dim3 grid((unsigned)blocks), block(NT * KW);
+  if (buf == kDwords)
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, PF, kDwords, KW>), grid, block, 0, s, a);
+  else if (DT != kF32 && buf == kOdd)
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, DT == kF32 ? kAny : kOdd, KW>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, false, KW>), dim3((unsigned)blocks), dim3(NT * KW), 0,
-                       s, a);
+    hipLaunchKernelGGL((gemm_grouped<DT, RED, B_KC, BM, BN, WR, 1, kAny, KW>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
@@ -388,7 +403,7 @@ inline double tile_time(double tiles, double alone, double full, int per) {
 inline double large_time(double tiles) { return 1.5 * ceil(tiles / 256.0); }
 
 template <int DT, bool B_KC>
-hipError_t launch_rows(const GroupArgs& a, bool buf, bool large, hipStream_t s) {
+hipError_t launch_rows(const GroupArgs& a, int buf, bool large, hipStream_t s) {
   // Rows a group has on average: a tile taller than that computes rows that
   // no group has, one shorter reads the weights once more for each tile.
   const int avg = (a.T + a.E - 1) / a.E;
@@ -425,7 +440,7 @@ hipError_t launch_rows(const GroupArgs& a, bool buf, bool large, hipStream_t s) 
 }
 
 template <int DT>
-hipError_t launch_reduce(const GroupArgs& a, bool buf, bool large, hipStream_t s) {
+hipError_t launch_reduce(const GroupArgs& a, int buf, bool large, hipStream_t s) {
   if constexpr (DT == kF32) {
     return launch<DT, true, false, 64, 64, 2, 2>(a, buf, s);
   } else {
@@ -445,8 +460,9 @@ hipError_t launch_reduce(const GroupArgs& a, bool buf, bool large, hipStream_t s
 
 // Buffer loads take any multiple of 4 bytes; their offsets stay below 2^31 in 128
 // rows (KC) or 64 k (KS) of an operand.
-static bool buf_ok(const void* p, long long ld, long long batch, int es) {
-  return (uintptr_t)p % 4 == 0 && ld * es % 4 == 0 && batch * es % 4 == 0 && ld * es <= (1ll << 23);
+static int loads_of(const void* p, long long ld, long long batch, int es) {
+  if (ld * es > (1ll << 23)) return kgrp::kAny;
+  return (uintptr_t)p % 4 == 0 && ld * es % 4 == 0 && batch * es % 4 == 0 ? kgrp::kDwords : kgrp::kOdd;
 }
 
 hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
@@ -471,7 +487,8 @@ hipError_t grouped_gemm(const GroupedProblem& p, hipStream_t stream) {
   a.sB = p.sB;
   a.sC = p.sC;
   a.zero_tail = p.zero_tail;
-  const bool buf = buf_ok(p.A, p.lda, 0, es) && buf_ok(p.B, p.ldb, p.sB, es);
+  const int la = loads_of(p.A, p.lda, 0, es), lb = loads_of(p.B, p.ldb, p.sB, es);
+  const int buf = la == kgrp::kAny || lb == kgrp::kAny ? kgrp::kAny : la == lb ? la : kgrp::kOdd;
   const bool large = p.dtype != kF32 && grouped_w4_ok(a, red, p.b_colmajor);
   switch (p.dtype) {
     case kF32:

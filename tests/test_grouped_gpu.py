@@ -393,3 +393,43 @@ def test_capture_beside_a_living_eager_graph_is_refused(strided):
         graph.replay()
         with torch.no_grad():
             assert torch.equal(y, ops.grouped_matmul(x, w, ends))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("colmajor", [False, True], ids=["row", "col"])
+@pytest.mark.parametrize("sizes,K,N", [
+    ([5, 0, 7, 65, 3], 33, 17), ([130, 61, 9], 129, 257), ([41] * 3, 1001, 127), ([300, 5], 64, 65),
+    ([1, 2], 1, 3), ([63, 0, 1], 127, 128), ([3], 2049, 31)])
+def test_odd_strides(dtype, colmajor, sizes, K, N):
+    """Contiguous operands of odd widths at odd elements, with NaN right before and behind them, and
+    in turn in the rows of every other expert; nothing is written beside the result."""
+    dt, T, E = DT[dtype], sum(sizes), len(sizes)
+
+    def place(t):
+        b = torch.full((t.numel() + 4,), float("nan"), device="cuda", dtype=t.dtype)
+        b[1:1 + t.numel()] = t.reshape(-1)
+        return b[1:1 + t.numel()].view(t.shape)
+
+    x0, w0 = _data(T, K, N, E, dt)
+    dy0, _ = _data(T, N, 1, 1, dt, seed=3)
+    ends = _ends(sizes)
+    x, dy = place(x0), place(dy0)
+    w = place(w0.transpose(1, 2)).transpose(1, 2) if colmajor else place(w0)
+    b = torch.full((T * N + 3,), 3.0, device="cuda", dtype=dt)
+    out = ops.grouped_matmul(x, w, ends, out=b[1:1 + T * N].view(T, N))
+    _close(out, _rows_exact(x0, w0, ends), _rows_exact(x0.abs(), w0.abs(), ends), K)
+    assert bool((b[:1] == 3).all()) and bool((b[1 + T * N:] == 3).all())
+    wt = w0.transpose(1, 2)
+    _close(ops.grouped_matmul(dy, w.transpose(1, 2), ends), _rows_exact(dy0, wt, ends),
+           _rows_exact(dy0.abs(), wt.abs(), ends), N)
+    exact, mag = _reduce_exact(x0, dy0, ends), _reduce_exact(x0.abs(), dy0.abs(), ends)
+    b = torch.full((E * K * N + 3,), 3.0, device="cuda", dtype=dt)
+    dw = ops.grouped_weight_grad(x, dy, ends, out=b[1:1 + E * K * N].view(E, K, N))
+    _close(dw, exact, mag, max(sizes))
+    assert bool((b[:1] == 3).all()) and bool((b[1 + E * K * N:] == 3).all())
+    lo = 0
+    for e, n in enumerate(sizes):
+        xe, dye = place(torch.full_like(x0, float("nan"))), place(torch.full_like(dy0, float("nan")))
+        xe[lo:lo + n], dye[lo:lo + n] = x0[lo:lo + n], dy0[lo:lo + n]
+        _close(ops.grouped_weight_grad(xe, dye, ends)[e], exact[e], mag[e], n)
+        lo += n
