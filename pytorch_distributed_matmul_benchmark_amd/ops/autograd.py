@@ -4,8 +4,8 @@ differentiable ops.
 Forward ``C = A @ B`` and both backward GEMMs (``dA = dC @ Bᵀ``,
 ``dB = Aᵀ @ dC``) run on the native kernels; transposed operands are
 materialised row-major first (the kernels take row-major NN operands with a
-unit inner stride). Lets the benchmark GEMM drop into a training step
-(used by ``__graft_entry__.smoke``).
+unit inner stride; the grouped products read a transposed weight in place). Lets the
+benchmark GEMM drop into a training step (used by ``__graft_entry__.smoke``).
 """
 from __future__ import annotations
 
