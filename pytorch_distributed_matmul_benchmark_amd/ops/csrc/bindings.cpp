@@ -338,9 +338,10 @@ bool rows_ok(const at::Tensor& t, int64_t* ld) {
   return (cols <= 1 || t.stride(-1) == 1) && *ld >= cols;
 }
 
+// (the kernels add two sizes, or a tile's to one, in 32 bits)
 bool fits(std::initializer_list<int64_t> sizes) {
   for (int64_t v : sizes)
-    if (v > INT32_MAX) return false;
+    if (v > (1 << 30)) return false;
   return true;
 }
 

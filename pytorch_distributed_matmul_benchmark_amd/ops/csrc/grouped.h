@@ -114,6 +114,7 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, unsigned b, int la
     const int tot = __builtin_amdgcn_readlane(inc, 63);
     if (slot < base + tot) break;
     base += tot;
+    if (c0 > a.E) return false;  // (only if `ends` is written meanwhile: the search ends all the same)
     if (c0 == 0) carry = group_end(a.ends, a.ends64, a.T, min(63, a.E - 1));
     c0 += 64;
     l = lane_group<BM>(a, c0, lane, carry);

@@ -37,7 +37,7 @@ def _native_call(name: str, x, *args):
 
 def _must(out: Optional[torch.Tensor], op: str) -> torch.Tensor:
     if out is None:
-        raise ValueError(f"{op}: out must have contiguous rows that do not overlap, and sizes below 2^31")
+        raise ValueError(f"{op}: out must have contiguous rows that do not overlap, and sizes up to 2^30")
     return out
 
 

@@ -433,3 +433,59 @@ def test_odd_strides(dtype, colmajor, sizes, K, N):
         xe[lo:lo + n], dye[lo:lo + n] = x0[lo:lo + n], dy0[lo:lo + n]
         _close(ops.grouped_weight_grad(xe, dye, ends)[e], exact[e], mag[e], n)
         lo += n
+
+
+def test_captured_training_step():
+    """Forward and backward pass in one graph, replayed with other rows, weights and sizes beside
+    eager work of the same kind."""
+    T, K, N, E = 700, 256, 192, 5
+    x, w = (t.requires_grad_() for t in _data(T, K, N, E, torch.bfloat16))
+    dy, _ = _data(T, N, 1, 1, torch.bfloat16, seed=9)
+    ends = _ends([100, 0, 300, 200, 60])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.native_grouped_matmul(x, w, ends), (x, w), dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.native_grouped_matmul(x, w, ends)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+    for i, sizes in enumerate([[100, 0, 300, 200, 60], [0, 0, 0, 0, 700], [140] * 5, [1, 2, 3, 4, 5]]):
+        x0, w0 = _data(T, K, N, E, torch.bfloat16, seed=20 + i)
+        with torch.no_grad():
+            x.copy_(x0), w.copy_(w0), ends.copy_(_ends(sizes))
+        graph.replay()
+        with torch.no_grad():
+            assert torch.equal(y, ops.grouped_matmul(x0, w0, ends))
+            assert torch.equal(dx, ops.grouped_matmul(dy, w0.transpose(1, 2), ends))
+            assert torch.equal(dw, ops.grouped_weight_grad(x0, dy, ends))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_offsets_past_32_bits(few):
+    """Rows, weights and gradients of more than 4 GiB: the far ends."""
+    K, dt = 16384, torch.bfloat16
+    T, E = (20, 70) if few else (140000, 2)
+    x = torch.empty(T, K, device="cuda", dtype=dt).normal_()
+    w = torch.empty(E, K, 2048 if few else 40, device="cuda", dtype=dt).normal_()
+    at = [10, 20] if few else [1, T - 3]
+    ends = torch.tensor([0] * (E - 2) + at, device="cuda")
+    y = ops.grouped_matmul(x, w, ends)
+    rows = torch.tensor([0, 9, 10, 19] if few else [0, 1, 2, T - 300, T - 5, T - 4], device="cuda")
+    for r in rows.tolist():
+        e = E - 2 if r < at[0] else E - 1
+        xr, we = x[r:r + 1].double(), w[e].double()
+        _close(y[r:r + 1], xr @ we, xr.abs() @ we.abs(), K)
+    if not few:
+        assert bool((y[T - 3:] == 0).all())
+    del w, y
+    T = 40
+    x, dy = x[:T].contiguous(), torch.randn(x[:T].shape[0], 24584, device="cuda").to(dt)
+    ends = torch.tensor([0] * 10 + [x.shape[0] // 2, x.shape[0]], device="cuda")
+    dw = ops.grouped_weight_grad(x, dy, ends)  # 12 x 16384 x 24584
+    half = x.shape[0] // 2
+    xs, ds = x[half:, K - 70:].double(), dy[half:, -70:].double()
+    _close(dw[11, K - 70:, -70:], xs.t() @ ds, xs.abs().t() @ ds.abs(), half)
+    assert not bool(dw[:10, ::1000].any())

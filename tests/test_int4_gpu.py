@@ -152,3 +152,17 @@ def test_quantised_weight_end_to_end():
     for sym in (False, True):
         q, s, z = ops.int4_quantize(w, 128, sym)
         _close(ops.int4_matmul(x, q, s, z), x, *_values(q, s, z), 4)
+
+
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_offsets_past_32_bits(T):
+    """Expert weights of more than 4 GiB: the last expert's last columns."""
+    E, N, K, G = 5, 131080, 16384, 128
+    q = torch.empty(E, N, K // 2, device="cuda", dtype=torch.uint8).random_(0, 256)
+    s = torch.full((E, N, K // G), 0.01, device="cuda", dtype=torch.float16)
+    s[:, -3:] = 0.02
+    x = torch.randn(T, K, device="cuda").half()
+    ends = torch.tensor([0, 0, 0, T // 2, T], device="cuda")
+    y = ops.int4_matmul(x, q, s, ends=ends)
+    for e, rows in ((3, slice(0, T // 2)), (4, slice(T // 2, T))):
+        _close(y[rows, -40:], x[rows], *_values(q[e, -40:], s[e, -40:], None), K // G)
