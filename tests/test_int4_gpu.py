@@ -166,3 +166,13 @@ def test_offsets_past_32_bits(T):
     y = ops.int4_matmul(x, q, s, ends=ends)
     for e, rows in ((3, slice(0, T // 2)), (4, slice(T // 2, T))):
         _close(y[rows, -40:], x[rows], *_values(q[e, -40:], s[e, -40:], None), K // G)
+
+
+@pytest.mark.parametrize("G,zero", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("M", [1, 4, 13])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_long_sums_of_many_columns(dtype, M, G, zero):
+    N, K = 8300, 6272 if G == 128 else 6240 if G == 32 else 6208
+    q, s, z = _weight((), N, K, G, DT[dtype], zero)
+    x = torch.randn(M, K, device="cuda").to(DT[dtype])
+    _close(ops.int4_matmul(x, q, s, z), x, *_values(q, s, z), K // G)
