@@ -428,6 +428,11 @@ hipError_t launch_rows(const GroupArgs& a, int buf, bool large, hipStream_t s) {
     // an MFMA of 4 k takes as long as one of 32 in 16 bits: small tiles lose nothing to
     // loads, and pad groups and widths less (8 experts of 512 rows, 2048 x 2048: 32 x 64
     // 306 us, 64 x 64 315, 64 x 128 345, 128 x 128 402; 16 of 85, 1001 x 1416: 53, 60, 75)
+    // few tiles, as above (621 rows of 9, 2048 x 256: 34 us alone, 24 in 4 sets; 800 of 6, 1536 x 512: 26, 20;
+    // in 2 sets: 1150 of 4, 704 x 512 20, 18)
+    const double t32 = row_tiles(a, 32) * ((a.N + 63) / 64);
+    if (long_sum && t32 <= 160) return launch<DT, false, B_KC, 32, 64, 2, 2, 4>(a, buf, s);
+    if (long_sum && t32 <= 320) return launch<DT, false, B_KC, 32, 64, 2, 2, 2>(a, buf, s);
     if (avg <= 256) return launch<DT, false, B_KC, 32, 64, 2, 2>(a, buf, s);
     return launch<DT, false, B_KC, 64, 64, 2, 2>(a, buf, s);
   } else {
@@ -440,6 +445,10 @@ hipError_t launch_rows(const GroupArgs& a, int buf, bool large, hipStream_t s) {
     const double t128 = tile_time(row_tiles(a, 128) * n128, 0.87, 1.83, 2);
     if (large && large_time(row_tiles(a, 256) * n256) <= (t64 < t128 ? t64 : t128))
       return grouped_w4(a, DT, false, B_KC, s);
+    // few tiles again (1000 rows of 4, 4096 x 512: 64 rows a tile 37 us, in 2 sets 27, 32 rows in 4 sets 20; 529
+    // of 6, 2496 x 1344: 22.8, 19.3, 15.5; 150 of 4, 1024 x 2048: 11.8, -, 8.7)
+    if (long_sum && row_tiles(a, 32) * n128 <= 256) return launch<DT, false, B_KC, 32, 128, 1, 1, 4>(a, buf, s);
+    if (long_sum && row_tiles(a, 64) * n128 <= 256) return launch<DT, false, B_KC, 64, 128, 2, 1, 2>(a, buf, s);
     if (t64 < t128) return launch<DT, false, B_KC, 64, 128, 2, 1>(a, buf, s);
     return launch<DT, false, B_KC, 128, 128, 2, 1>(a, buf, s);
   }
@@ -448,6 +457,9 @@ hipError_t launch_rows(const GroupArgs& a, int buf, bool large, hipStream_t s) {
 template <int DT>
 hipError_t launch_reduce(const GroupArgs& a, int buf, bool large, hipStream_t s) {
   if constexpr (DT == kF32) {
+    // (2048 rows of 4, 256 x 512: one set of waves 15.0 us, 2 13.5; 4096 of 8: 15.8, 14.7)
+    if (a.T >= 256ll * a.E && (double)a.E * ((a.M + 63) / 64) * ((a.N + 63) / 64) <= 256)
+      return launch<DT, true, false, 64, 64, 2, 2, 2>(a, buf, s);
     return launch<DT, true, false, 64, 64, 2, 2>(a, buf, s);
   } else {
     // As above, with what a tile costs beside its 64-k steps: large ones 5 us, 128 x 128
@@ -458,6 +470,9 @@ hipError_t launch_reduce(const GroupArgs& a, int buf, bool large, hipStream_t s)
     const double t128 = (double)a.E * ((a.M + 127) / 128) * ((a.N + 127) / 128);
     const double small = t128 <= 256 ? 0.87 * nk + 3 : (1.83 * nk + 1.5) * (t128 <= 512 ? 1.0 : t128 / 512);
     if (large && (1.5 * even + 5) * ceil(t256 / 256) <= small) return grouped_w4(a, DT, true, false, s);
+    // (4096 rows of 4, 512 x 512: one set of waves 16.6 us, 2 14.6; 8192 of 4, 1024 x 1024: 30.5, 27.3; but
+    // 4096 of 8, 512 x 768: 11.8, 12.9)
+    if (nk >= 12 && t128 <= 256) return launch<DT, true, false, 128, 128, 2, 1, 2>(a, buf, s);
     return launch<DT, true, false, 128, 128, 2, 1>(a, buf, s);
   }
 }

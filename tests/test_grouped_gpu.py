@@ -489,3 +489,28 @@ def test_offsets_past_32_bits(few):
     xs, ds = x[half:, K - 70:].double(), dy[half:, -70:].double()
     _close(dw[11, K - 70:, -70:], xs.t() @ ds, xs.abs().t() @ ds.abs(), half)
     assert not bool(dw[:10, ::1000].any())
+
+
+# sums long enough, and tiles few enough, that several sets of waves share a tile's sum
+@pytest.mark.parametrize("sizes,K,N", [
+    ([300, 0, 299, 5], 1090, 1100), ([300, 0, 299, 5], 1091, 2100), ([300, 0, 299, 5], 1104, 330),
+    ([300, 0, 299, 5], 1600, 700), ([40, 1, 33, 64, 39, 80], 2056, 257)])
+@pytest.mark.parametrize("colmajor", [False, True], ids=["row", "col"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_few_tiles_of_long_sums(dtype, colmajor, sizes, K, N):
+    x, w = _data(sum(sizes) + 2, K, N, len(sizes), DT[dtype], colmajor)
+    x[sum(sizes):] = float("nan")
+    ends = _ends(sizes)
+    y = ops.grouped_matmul(x, w, ends)
+    x[sum(sizes):] = 0
+    _close(y, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
+
+
+@pytest.mark.parametrize("sizes,M,N", [([2000, 3, 1500], 136, 200), ([1023, 0, 1, 900, 2200], 300, 131)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_few_gradients_of_long_sums(dtype, sizes, M, N):
+    x, _ = _data(sum(sizes), M, 1, 1, DT[dtype])
+    dy, _ = _data(sum(sizes), N, 1, 1, DT[dtype], seed=5)
+    ends = _ends(sizes)
+    dw = ops.grouped_weight_grad(x, dy, ends)
+    _close(dw, _reduce_exact(x, dy, ends), _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
