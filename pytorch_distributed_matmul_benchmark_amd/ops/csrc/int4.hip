@@ -28,8 +28,8 @@
 //
 // Two kernels: gemm_int4_few for 16 rows a tile and short sums or narrow weights, and
 // gemm_int4_rows for more, where the rows of a block come through LDS once for 64 columns.
-// What bounds them: 1 row, 8192 x 16384: 15 us, the read of the weight (4.5 TB/s) with 7 us of
-// widening beside it; 16 rows, 4096 x 11007, groups of 32: 11.7 us, of which the vector
+// What bounds them: 1 row, 8192 x 16384: 14.7 us, the read of the weight (4.7 TB/s) with 7 us of
+// widening beside it; 16 rows, 4096 x 11007, groups of 32: 11.4 us, of which the vector
 // units work 5.3 (36 instructions for an MFMA) and the rest is launch, first loads and the
 // join; 100 rows, 4096 x 8192: 21.5 us, vector units 9.5, matrix units 7 (two products for
 // a bf16 weight) and LDS 5, which overlap little with a barrier a step.
