@@ -377,7 +377,7 @@ __device__ __forceinline__ void few_sums(const Args& a, const RowTile& r, int n0
 // (Scheduled for four waves a SIMD, which is what a grid has of it: 64 experts 2048 x 2048 of 64 rows
 // 27.3 -> 25.2 us, 16 x 4096 x 11007 12.8 -> 12.3.)
 template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
-__attribute__((amdgpu_waves_per_eu(4, 4)))
+__attribute__((amdgpu_waves_per_eu(NB > 1 && SG > 1 ? 2 : 4, 4)))
 __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
   constexpr int KB = 64;  // chunks whose scales are in LDS
   using SB = ScaleBlock<DT, 16 * NB, SG, KB, ZERO, 64 * W>;
