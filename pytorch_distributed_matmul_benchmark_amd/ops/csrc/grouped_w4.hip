@@ -445,7 +445,8 @@ __global__ void __launch_bounds__(NT, 1) gemm_grouped_w4(GroupArgs a) {
     ktile<DT, 0, 48, 48, true, true>(c, cur, nxt, more, smem, 0, acc, A, A7a, A7b, B0, B1);
     ktile<DT, 1, 48, 16, false, true>(c, cur, nxt, more, smem, 1, acc, A, A7b, A7a, B1, B0);
     int t = 2;
-    for (; t + 6 <= cur.nk; t += 2) {
+    // (fetches up to B's K-tile t + 4: it has to lie before the sum's last two)
+    for (; t + 8 <= cur.nk; t += 2) {
       ktile<DT, 0, 16, 16, false, false>(c, cur, nxt, more, smem, t, acc, A, A7a, A7b, B0, B1);
       ktile<DT, 1, 16, 16, false, false>(c, cur, nxt, more, smem, t + 1, acc, A, A7b, A7a, B1, B0);
     }

@@ -1,0 +1,62 @@
+"""Expert-grouped products where a sum ends inside a K-tile, beside what must not reach it."""
+import pytest
+import torch
+from test_grouped_gpu import DT, _close, _data, _ends, _reduce_exact, _rows_exact
+
+from pytorch_distributed_matmul_benchmark_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _beside_nan(t):
+    """t with 16 bytes of NaN behind every row."""
+    b = torch.full((*t.shape[:-1], t.shape[-1] + 8), float("nan"), device="cuda", dtype=t.dtype)
+    b[..., :-8] = t
+    return b[..., :-8]
+
+
+# K-tiles of 64 on the large tiles: 7, 9, 13 and 23, the last one of 8 to 56 k
+@pytest.mark.parametrize("K", [392, 424, 552, 776, 1416])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_large_tiles_end_inside_a_k_tile(dtype, K):
+    """All three products of a layer whose sums are K long, on the large tiles, with NaN beside every row."""
+    dt, T, wide, sizes = DT[dtype], 4096, 2048, [2100, 1996]
+
+    ends = _ends(sizes)
+    # y = x @ w, column-major weights
+    x, w = _data(T, K, wide, 2, dt, colmajor=True)
+    got = ops.grouped_matmul(_beside_nan(x), _beside_nan(w.transpose(1, 2)).transpose(1, 2), ends)
+    _close(got, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
+    # dx = dy @ w^T, row-major weights of K columns; dw of K columns
+    x, w = _data(T, wide, K, 2, dt)
+    dy, _ = _data(T, K, 1, 1, dt, seed=3)
+    xs, ws = _beside_nan(x).requires_grad_(), _beside_nan(w).requires_grad_()
+    dx, dw = torch.autograd.grad(ops.native_grouped_matmul(xs, ws, ends), (xs, ws), _beside_nan(dy))
+    wt = w.transpose(1, 2)
+    _close(dx, _rows_exact(dy, wt, ends), _rows_exact(dy.abs(), wt.abs(), ends), K)
+    _close(dw, _reduce_exact(x, dy, ends), _reduce_exact(x.abs(), dy.abs(), ends), max(sizes))
+
+
+def test_an_infinite_weight_stays_in_its_column_of_the_large_tiles():
+    T, K, N = 4096, 424, 2048
+    x, w = _data(T, K, N, 2, torch.bfloat16, colmajor=True)
+    ends = _ends([2000, 2096])
+    clean = ops.grouped_matmul(x, w, ends)
+    w[1, :56, 700] = float("inf")  # contiguous columns: right behind column 699's last k
+    y = ops.grouped_matmul(x, w, ends)
+    assert not bool(y[2000:, 700].isfinite().any())
+    y[2000:, 700] = clean[2000:, 700]
+    assert torch.equal(y, clean)
+
+
+@pytest.mark.parametrize("K", [520, 1416])
+def test_large_tiles_of_ragged_experts_end_inside_a_k_tile(K):
+    """Tiles of several experts in one stream: the K-tile that ends a sum is fetched while the tile before it,
+    another expert's, is multiplied."""
+    sizes = [700, 0, 513, 1, 900, 1100, 300]
+    x, w = _data(sum(sizes) + 30, K, 2568, len(sizes), torch.bfloat16, colmajor=True)
+    x[sum(sizes):] = float("nan")
+    ends = _ends(sizes)
+    y = ops.grouped_matmul(x, _beside_nan(w.transpose(1, 2)).transpose(1, 2), ends)
+    x[sum(sizes):] = 0
+    _close(y, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
