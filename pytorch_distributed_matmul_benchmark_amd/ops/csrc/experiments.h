@@ -62,8 +62,7 @@ static int experiment_resolve(const Problem& p, int kernel, bool fast, bool w4, 
     case kF32_256: case kF32NoDma: case kF32_256sDirect: case kF32_256p: return f32fast ? kernel : -1;
     case kT128Unfused: return t128 ? kernel : -1;
     case kF32T128B32: return p.dtype == kF32 && supports(p, kF32T128) ? kernel : -1;
-    case kF32W4S: case kF32W4SDbg:
-      return f32fast && gemm_f32_w4s_fits(shape_args(p)) && device_cus() % 8 == 0 ? kernel : -1;
+    case kF32W4S: case kF32W4SDbg: return -1;  // not launched: its first launch has hung, cause unknown
     case kF32T128Lean: case kF32T128x2Lean: case kF32T64Lean: case kF32T64x2Lean:
       return p.dtype == kF32 && supports(p, kF32T128) && gemm_f32_tile_ln_fits(shape_args(p)) ? kernel : -1;
     case kF32W4B32: case kF32W4NB: case kF32W4NBP: case kF32W4NoDma: case kF32W4NoFrag:
@@ -181,12 +180,7 @@ static hipError_t experiment_launch(const Problem& p, int k, const GemmArgs& a, 
     case kF32_256sDirect: return gemm_f32_256_launch(a, 10, stream);
     case kF32_256p: return gemm_f32_256_launch(a, 11, stream);
     case kF32T128B32: return tiled_launch(p, kF32T128, a, p.workspace, p.workspace_bytes, stream, 1);
-    case kF32W4S: case kF32W4SDbg: {
-      GemmArgs s = a;
-      s.splitk = 1;
-      s.pers_grid = ((p.cus > 0 ? p.cus : device_cus()) / 8) * 8;
-      return gemm_f32_w4_launch(s, stream, k == kF32W4S ? 14 : 15);
-    }
+    case kF32W4S: case kF32W4SDbg: return hipErrorNotSupported;
     case kF32T128Lean: case kF32T128x2Lean: case kF32T64Lean: case kF32T64x2Lean:
       return tiled_launch(p, ln_base(k), a, p.workspace, p.workspace_bytes, stream, 5 + (k - kF32T128Lean));
     case kF32W4B32: return tiled_launch(p, kF32W4, a, p.workspace, p.workspace_bytes, stream, 1);

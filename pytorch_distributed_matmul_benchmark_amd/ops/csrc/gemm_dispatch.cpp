@@ -29,7 +29,6 @@ hipError_t gemm_generic_launch(int dt, GemmArgs a, bool vec, hipStream_t stream)
 bool gemm_f32_256_supported(const GemmArgs& a, size_t align_a, size_t align_b, size_t align_c);
 hipError_t gemm_f32_256_launch(GemmArgs a, int variant, hipStream_t stream);
 hipError_t gemm_f32_w4_launch(GemmArgs a, hipStream_t stream, int variant);
-bool gemm_f32_w4s_fits(const GemmArgs& a);  // experiments build: kF32W4S
 bool gemm_f32_w4l_fits(const GemmArgs& a);
 bool gemm_w4s_lean_fits(const GemmArgs& a);  // experiments build: kMfmaW4SLean
 bool gemm_f32_tile_supported(const GemmArgs& a, size_t align_a, size_t align_b, size_t align_c);
