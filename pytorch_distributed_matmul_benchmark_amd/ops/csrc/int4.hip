@@ -7,13 +7,17 @@
 // a weight is never rounded. Two values at a time, at one place of a dword's
 // halves, become B + q (a power of two B whose mantissa step fits the place) by
 // one and-or, most after one shift:
-//   bf16  B = 128 for nibble 0 (bits 0-3 as they are), 16 for the others (shifted to bits 3-6)
+//   bf16  B = 16: every nibble shifted to bits 3-6
 //   fp16  B = 1024: nibbles 0 and 2 at bits 0-3, 1 and 3 at bits 4-7 (16 times the value)
 // fp16 then subtracts B + zero exactly (v_pk_add_f16, for bits 4-7 v_pk_fma_f16 with
 // 1/16); bf16, which has no packed add, adds a second product with the constants
-// -(B + zero), also whole numbers, to the same fp32 sum. Each group's fp32 sum is
-// scaled once, in fp32. (A row of X with an infinity gives NaN in bf16: the two
-// products cancel.)
+// -(16 + zero), also whole numbers, to the same fp32 sum. Each group's fp32 sum is
+// scaled once, in fp32.
+//
+// So a bf16 sum's terms are x (16 + q) and -x (16 + zero), not x (q - zero): its fp32 error is relative to
+// |x| (32 + q + zero) (B = 128 for nibble 0, which needs no shift, is one instruction in 36 less and
+// made that up to nine times as much), a row whose 31 sum |x| over a group passes 3.4e38 gives NaN, and so
+// does a row with an infinity: the two products cancel.
 //
 // Loads: an MFMA operand has its 16 columns in neighbouring lanes, but 16-byte
 // loads whose neighbours are in 16 rows of memory look a cache line up for
@@ -74,22 +78,23 @@ struct Bits {
   unsigned mask0, mask1, or0, or1;
   template <int DT>
   __device__ static __forceinline__ Bits make() {
-    Bits b = DT == kBF16 ? Bits{0x000f000fu, 0x00780078u, 0x43004300u, 0x41804180u}
+    Bits b = DT == kBF16 ? Bits{0u, 0x00780078u, 0u, 0x41804180u}
                          : Bits{0x000f000fu, 0x00f000f0u, 0x64006400u, 0x64006400u};
-    asm("" : "+s"(b.mask0), "+s"(b.mask1), "+v"(b.or0), "+v"(b.or1));
+    asm("" : "+s"(b.mask1), "+v"(b.or1));
+    if constexpr (DT != kBF16) asm("" : "+s"(b.mask0), "+v"(b.or0));
     return b;
   }
 };
 
-// What widen() subtracts for a zero point, two halves each: [0] -(B + zero) of the first pair,
-// [1] of the others. fp16: [1] -(64 + zero), after the 1/16.
+// What widen() subtracts for a zero point, two halves each. bf16: -(16 + zero). fp16: [0] -(B + zero) of the
+// first pair, [1] of the others -(64 + zero), after the 1/16.
 struct Minus {
   unsigned m[2];
 };
 template <int DT>
 __device__ __forceinline__ Minus minus_of(unsigned z) {
-  // (bf16 128 + z: step 1 at bit 0, 16 + z: bit 3; fp16 1024 + z: bit 0, 64 + z: bit 4)
-  return DT == kBF16 ? Minus{{z * 0x00010001u + 0xc300c300u, z * 0x00080008u + 0xc180c180u}}
+  // (bf16 16 + z: step 1 at bit 3; fp16 1024 + z: bit 0, 64 + z: bit 4)
+  return DT == kBF16 ? Minus{{z * 0x00080008u + 0xc180c180u, z * 0x00080008u + 0xc180c180u}}
                      : Minus{{z * 0x00010001u + 0xe400e400u, z * 0x00100010u + 0xd400d400u}};
 }
 
@@ -98,7 +103,7 @@ template <int DT>
 __device__ __forceinline__ s16x8 widen(unsigned d, const Bits& b, const Minus& minus) {
   u32x4 v;
   if constexpr (DT == kBF16) {
-    v = u32x4{(d & b.mask0) | b.or0, ((d >> 1) & b.mask1) | b.or1, ((d >> 5) & b.mask1) | b.or1,
+    v = u32x4{((d << 3) & b.mask1) | b.or1, ((d >> 1) & b.mask1) | b.or1, ((d >> 5) & b.mask1) | b.or1,
               ((d >> 9) & b.mask1) | b.or1};
   } else {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

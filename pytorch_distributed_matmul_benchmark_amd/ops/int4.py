@@ -116,7 +116,13 @@ def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
     ``ends`` [E] and a weight for each expert (``q`` [E, N, K/2]) the rows are grouped
     as in ``grouped_matmul``: rows behind the last expert's are zero in a fresh
     result and left as they were in ``out``. The weight is frozen: no gradients
-    are recorded. In bfloat16 a row with an infinity gives NaN."""
+    are recorded.
+
+    Bfloat16 rows are multiplied by ``16 + q`` and ``-(16 + zero)``, whose fp32 sums then
+    cancel: their error is relative to ``scale * sum(|x| (32 + q + zero))``, so a value some
+    1e5 times as large as the rest of its row leaves noise there even where its weight is zero,
+    and a row gives NaN if it holds an infinity or if 31 times the sum of its magnitudes
+    over a group passes 3.4e38. (float16 rows are multiplied by ``q - zero``.)"""
     op = "int4_matmul"
     res = _native_call("int4_matmul", x, q, scale, zero, ends, out)
     if res is not None:

@@ -1,0 +1,43 @@
+"""4-bit products of whole numbers, where every fp32 sum is exact: compared bit for bit with the
+64-bit result rounded once."""
+import pytest
+import torch
+from test_int4_gpu import DT, _values, _weight
+
+from pytorch_distributed_matmul_benchmark_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(y, x, q, s, z):
+    want = (x.double() @ _values(q, s, z)[0].t()).to(y.dtype)
+    assert torch.equal(y, want), f"{(y != want).sum().item()} of {y.numel()} differ"
+
+
+@pytest.mark.parametrize("M", [1, 20, 100])
+@pytest.mark.parametrize("zero", [False, True], ids=["sym", "zero"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_an_outlier_of_zero_weights_leaves_no_trace(dtype, zero, M):
+    """One value of 2^18 (fp16: 2^15) a row, whose weights are zero, among whole numbers up to 3: every
+    product is below 31 x 2^18 and with the 255 others every sum below 2^23 + 255 x 3 x 31 < 2^24."""
+    K, N, big = 256, 200, 2.0 ** 18 if dtype == "bf16" else 2.0 ** 15
+    q, _, z = _weight((), N, K, 64, DT[dtype], zero)
+    s = torch.ones(N, K // 64, device="cuda", dtype=DT[dtype])
+    x = torch.randint(-3, 4, (M, K), device="cuda").to(DT[dtype])
+    nothing = (z if zero else torch.full_like(s, 8).byte()).repeat_interleave(32, -1)  # of each byte's group
+    at = torch.arange(M, device="cuda") % 16 + 16 * (torch.arange(M, device="cuda") % 7)  # each place of a dword
+    q[:, at // 2] = (nothing | nothing << 4)[:, at // 2]
+    x[torch.arange(M, device="cuda"), at] = big
+    y = ops.int4_matmul(x, q, s, z)
+    _same(y, x, q, s, z)
+
+
+def test_large_finite_rows():
+    """2^122 times a weight of up to 15: 31 x 2^122 is below the fp32 range's end, 3.4e38."""
+    K, N = 256, 96
+    q, s, z = _weight((), N, K, 128, torch.bfloat16, True)
+    s.fill_(2.0 ** -20)
+    x = torch.zeros(K, K, device="cuda", dtype=torch.bfloat16)
+    x.fill_diagonal_(2.0 ** 122)
+    for rows in (x[:1], x[:16], x):
+        _same(ops.int4_matmul(rows, q, s, z), rows, q, s, z)
