@@ -16,7 +16,7 @@
 //
 // So a bf16 sum's terms are x (16 + q) and -x (16 + zero), not x (q - zero): its fp32 error is relative to
 // |x| (32 + q + zero) (B = 128 for nibble 0, which needs no shift, is one instruction in 36 less and
-// made that up to nine times as much), a row whose 31 sum |x| over a group passes 3.4e38 gives NaN, and so
+// made that up to eight times as much), a row whose 31 sum |x| over a group passes 3.4e38 gives NaN, and so
 // does a row with an infinity: the two products cancel.
 //
 // Loads: an MFMA operand has its 16 columns in neighbouring lanes, but 16-byte

@@ -35,10 +35,12 @@ def _native_call(name: str, x, *args):
         return None
 
 
-def _must(out: Optional[torch.Tensor], op: str) -> torch.Tensor:
-    if out is None:
-        raise ValueError(f"{op}: out must have contiguous rows that do not overlap, and sizes up to 2^30")
-    return out
+def _must(res: Optional[torch.Tensor], out: Optional[torch.Tensor], op: str) -> torch.Tensor:
+    # (all else that a binding turns down has been checked or copied)
+    if res is None:
+        raise ValueError(f"{op}: sizes up to 2^30 only" if out is None else
+                         f"{op}: out must have contiguous rows that do not overlap, and sizes up to 2^30")
+    return res
 
 
 def _check_ends(ends: torch.Tensor, x: torch.Tensor, experts: int, op: str) -> None:
@@ -60,6 +62,8 @@ def _check_out(out: torch.Tensor, shape, like: torch.Tensor, op: str) -> None:
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{op}: out must be {tuple(shape)} {like.dtype} on {like.device}, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise RuntimeError(f"{op} records no gradient: out must not require one")
 
 
 def _no_grad(op: str, instead: str, *ts: torch.Tensor) -> None:
@@ -121,7 +125,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor,
             if hi > lo:
                 res[lo:hi] = torch.matmul(x[lo:hi], w[e])
         return res
-    return _must(_native_call("grouped_rows", _prep(x), _prep_weight(w), ends.contiguous(), out), op)
+    return _must(_native_call("grouped_rows", _prep(x), _prep_weight(w), ends.contiguous(), out), out, op)
 
 
 def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: torch.Tensor,
@@ -155,4 +159,4 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: torch.Tensor,
         for e, lo, hi in _ranges(ends, x.shape[0]):
             res[e] = torch.matmul(x[lo:hi].t(), dy[lo:hi])
         return res
-    return _must(_native_call("grouped_reduce", _prep(x), _prep(dy), ends.contiguous(), out), op)
+    return _must(_native_call("grouped_reduce", _prep(x), _prep(dy), ends.contiguous(), out), out, op)

@@ -24,6 +24,7 @@ from .gemm import _prep
 from .grouped import _check_ends, _check_out, _must, _native_call, _no_grad, _ranges
 
 INT4_DTYPES = (torch.float16, torch.bfloat16)
+MAX_K = 1 << 23  # of GPU tensors: K, and the distance of two rows that are read in place
 
 
 def _check_group(K: int, group: int, op: str) -> None:
@@ -100,9 +101,9 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` with 16-byte aligned rows, which the kernels load 16 bytes at a time (K is a
-    multiple of 32, so a copy is aligned)."""
+    multiple of 32, so a copy is aligned), at most 2^23 elements apart (a tile's rows are addressed in 32 bits)."""
     x = _prep(x)
-    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8):
+    if x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) > MAX_K)):
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -159,6 +160,8 @@ def int4_matmul(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
                 if hi > lo:
                     res[lo:hi] = torch.matmul(x[lo:hi].float(), w[e]).to(x.dtype)
         return res
+    if K > MAX_K:
+        raise ValueError(f"{op}: K = {K} (up to 2^23 on the GPU)")
     return _must(_native_call("int4_matmul", _rows(x), _plain(q), _plain(scale),
                               None if zero is None else _plain(zero),
-                              None if ends is None else ends.contiguous(), out), op)
+                              None if ends is None else ends.contiguous(), out), out, op)

@@ -1,0 +1,27 @@
+"""Expert-grouped and 4-bit products without a GPU: calls that are refused, and why."""
+import pytest
+import torch
+
+from pytorch_distributed_matmul_benchmark_amd import ops
+
+X, W, ENDS = torch.randn(4, 32), torch.randn(2, 32, 8), torch.tensor([1, 4])
+
+
+def _int4(x, **kw):
+    return ops.int4_matmul(x, *ops.int4_quantize(W[0].half(), 32), **kw)
+
+
+CALLS = {
+    "rows": lambda x=X, **kw: ops.grouped_matmul(x, W, ENDS, **kw),
+    "reduce": lambda x=X, **kw: ops.grouped_weight_grad(x, X, ENDS, **kw),
+    "int4": lambda x=X, **kw: _int4(x.half(), **kw),
+}
+
+
+@pytest.mark.parametrize("name", ["rows", "reduce", "int4"])
+def test_an_out_that_asks_for_gradients_is_refused(name):
+    out = torch.zeros_like(CALLS[name]())
+    with pytest.raises(RuntimeError, match="gradient"):
+        CALLS[name](out=out.clone().requires_grad_())
+    with torch.no_grad():
+        CALLS[name](out=out.requires_grad_())

@@ -41,3 +41,28 @@ def test_large_finite_rows():
     x.fill_diagonal_(2.0 ** 122)
     for rows in (x[:1], x[:16], x):
         _same(ops.int4_matmul(rows, q, s, z), rows, q, s, z)
+
+
+@pytest.mark.parametrize("ends", [False, True])
+def test_rows_far_apart(ends):
+    """The last tokens' rows of a batch of long sequences: more than 2^23 elements from row to row."""
+    K, N = 256, 96
+    q, s, z = _weight((2,) if ends else (), N, K, 64, torch.bfloat16, True)
+    far = torch.empty(3, 2049, 4096, device="cuda", dtype=torch.bfloat16)[:, -1, -K:]
+    far.copy_(torch.randn(3, K, device="cuda"))
+    assert far.stride(0) > 1 << 23
+    kw = {"ends": torch.tensor([1, 3], device="cuda")} if ends else {}
+    assert torch.equal(ops.int4_matmul(far, q, s, z, **kw), ops.int4_matmul(far.contiguous(), q, s, z, **kw))
+
+
+def test_refusals_name_their_reason():
+    K = (1 << 23) + 128
+    q = torch.zeros(1, K // 2, device="cuda", dtype=torch.uint8)
+    s = torch.ones(1, K // 128, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2\\^23"):
+        ops.int4_matmul(torch.zeros(1, K, device="cuda", dtype=torch.bfloat16), q, s)
+    q, s, x = q[:, :64].contiguous(), s[:, :1].contiguous(), torch.zeros(2, 128, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="do not overlap"):
+        ops.int4_matmul(x, q, s, out=torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(2, 1))
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.int4_matmul(x, q, s, out=torch.zeros(2, 1, device="cuda", dtype=torch.bfloat16, requires_grad=True))
