@@ -412,7 +412,8 @@ MaybeTensor grouped_reduce(const at::Tensor& x, const at::Tensor& dy, const at::
   if (!rows_ok(x, (int64_t*)&p.lda) || !rows_ok(dy, (int64_t*)&p.ldb)) return {};
   if (!output(out, {E, M, N}, x) || !rows_ok(*out, (int64_t*)&p.ldc)) return {};
   p.sC = out->stride(0);
-  if (E > 1 && p.sC < M * p.ldc) return {};
+  // the experts' matrices lie one after the other, or their rows in turn
+  if (E > 1 && M > 0 && p.sC < (M - 1) * p.ldc + N && (p.sC < N || (M > 1 && p.ldc < (E - 1) * p.sC + N))) return {};
   p.kind = pdmb::kGroupReduce;
   p.dtype = dtype_code(x.scalar_type());
   p.A = x.data_ptr();

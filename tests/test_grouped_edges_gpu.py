@@ -60,3 +60,20 @@ def test_large_tiles_of_ragged_experts_end_inside_a_k_tile(K):
     y = ops.grouped_matmul(x, _beside_nan(w.transpose(1, 2)).transpose(1, 2), ends)
     x[sum(sizes):] = 0
     _close(y, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), K)
+
+
+@pytest.mark.parametrize("T,M,N", [(9, 24, 40), (1500, 264, 520), (9, 1, 40), (9, 24, 1)])
+def test_weight_gradients_into_interleaved_matrices(T, M, N):
+    """out[e] as rows e, e + E, ... of one matrix: rows apart that do not overlap."""
+    x, _ = _data(T, M, 1, 1, torch.bfloat16)
+    dy, _ = _data(T, N, 1, 1, torch.bfloat16, seed=5)
+    ends = _ends([T // 2, 0, T - T // 2])
+    buf = torch.full((M, 3, N + 3), 5.0, device="cuda", dtype=torch.bfloat16)
+    out = buf[:, :, :N].transpose(0, 1)
+    assert ops.grouped_weight_grad(x, dy, ends, out=out) is out
+    assert torch.equal(out, ops.grouped_weight_grad(x, dy, ends)) and bool((buf[:, :, N:] == 5).all())
+    with pytest.raises(ValueError, match="overlap"):
+        ops.grouped_weight_grad(x, dy, ends, out=out[:1].expand(3, M, N))
+    if M > 1 and N > 1:
+        with pytest.raises(ValueError, match="overlap"):  # matrices one row apart
+            ops.grouped_weight_grad(x, dy, ends, out=buf.view(-1).as_strided((3, M, N), (N, N, 1)))
