@@ -345,8 +345,11 @@ bool fits(std::initializer_list<int64_t> sizes) {
   return true;
 }
 
+// (a tensor with a forward-mode tangent, which a result would drop silently)
+bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 bool records(const at::Tensor& a, const at::Tensor& b) {
-  return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+  return (at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad())) || dual(a) || dual(b);
 }
 
 // out as given, or a new one; false if it cannot be written as C.
@@ -356,7 +359,7 @@ bool output(c10::optional<at::Tensor>& out, at::IntArrayRef shape, const at::Ten
     return true;
   }
   return one_device(like, *out) && out->scalar_type() == like.scalar_type() && out->sizes() == shape &&
-         !(at::GradMode::is_enabled() && out->requires_grad());
+         !(at::GradMode::is_enabled() && out->requires_grad()) && !dual(*out);
 }
 
 using MaybeTensor = c10::optional<at::Tensor>;
@@ -449,6 +452,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     {
       at::AutoGradMode off(false);
       at::Tensor dy = grads[0];
+      TORCH_CHECK(!dual(dy), "native_grouped_matmul has no forward-mode derivative");
       int64_t ld;
       if (!rows_ok(dy, &ld)) dy = dy.contiguous();
       if (ctx->needs_input_grad(0)) {

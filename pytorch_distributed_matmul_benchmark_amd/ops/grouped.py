@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .gemm import SUPPORTED_DTYPES, _prep
@@ -64,12 +65,19 @@ def _check_out(out: torch.Tensor, shape, like: torch.Tensor, op: str) -> None:
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
     if torch.is_grad_enabled() and out.requires_grad:
         raise RuntimeError(f"{op} records no gradient: out must not require one")
+    _no_tangent(op, out)
 
 
 def _no_grad(op: str, instead: str, *ts: torch.Tensor) -> None:
-    # a result without a graph would drop the gradients silently
+    # a result without a graph or a tangent would drop the gradients silently
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
         raise RuntimeError(f"{op} records no gradient: {instead}")
+    _no_tangent(op, *ts)
+
+
+def _no_tangent(op: str, *ts: torch.Tensor) -> None:
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{op} has no forward-mode derivative")
 
 
 def _ranges(ends: torch.Tensor, rows: int):

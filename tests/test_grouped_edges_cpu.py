@@ -1,6 +1,7 @@
 """Expert-grouped and 4-bit products without a GPU: calls that are refused, and why."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from pytorch_distributed_matmul_benchmark_amd import ops
 
@@ -25,3 +26,21 @@ def test_an_out_that_asks_for_gradients_is_refused(name):
         CALLS[name](out=out.clone().requires_grad_())
     with torch.no_grad():
         CALLS[name](out=out.requires_grad_())
+
+
+def test_forward_mode_tangents_are_refused():
+    x, w = X.half(), W[0].half()
+    q, s, z = ops.int4_quantize(w, 32)
+    with fwAD.dual_level():
+        def dual(t):
+            return fwAD.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.grouped_matmul(dual(X), W, ENDS), lambda: ops.grouped_matmul(X, dual(W), ENDS),
+                     lambda: ops.grouped_weight_grad(dual(X), X, ENDS), lambda: ops.grouped_weight_grad(X, dual(X), ENDS),
+                     lambda: ops.grouped_matmul(X, W, ENDS, out=dual(torch.zeros(4, 8))),
+                     lambda: ops.int4_matmul(dual(x), q, s, z), lambda: ops.int4_matmul(x, q, dual(s), z),
+                     lambda: ops.native_grouped_matmul(dual(X), W, ENDS)):
+            with pytest.raises(RuntimeError, match="forward.mode|jvp"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward.mode|jvp"):
+                call()
+        assert ops.grouped_matmul(X, W, ENDS).shape == (4, 8)

@@ -1,6 +1,7 @@
 """Expert-grouped products where a sum ends inside a K-tile, beside what must not reach it."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from test_grouped_gpu import DT, _close, _data, _ends, _reduce_exact, _rows_exact
 
 from pytorch_distributed_matmul_benchmark_amd import ops
@@ -77,3 +78,22 @@ def test_weight_gradients_into_interleaved_matrices(T, M, N):
     if M > 1 and N > 1:
         with pytest.raises(ValueError, match="overlap"):  # matrices one row apart
             ops.grouped_weight_grad(x, dy, ends, out=buf.view(-1).as_strided((3, M, N), (N, N, 1)))
+
+
+def test_forward_mode_tangents_are_refused():
+    x, w, ends = torch.randn(4, 32, device="cuda"), torch.randn(2, 32, 8, device="cuda"), _ends([1, 3])
+    q, s, z = ops.int4_quantize(w[0].half(), 32)
+    leaf = x.clone().requires_grad_()
+    y = ops.native_grouped_matmul(leaf, w, ends)
+    with fwAD.dual_level():
+        def dual(t):
+            return fwAD.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.grouped_matmul(dual(x), w, ends), lambda: ops.grouped_matmul(x, dual(w), ends),
+                     lambda: ops.grouped_weight_grad(dual(x), x, ends), lambda: ops.grouped_weight_grad(x, dual(x), ends),
+                     lambda: ops.grouped_matmul(x, w, ends, out=dual(torch.zeros(4, 8, device="cuda"))),
+                     lambda: ops.int4_matmul(dual(x.half()), q, s, z), lambda: ops.int4_matmul(x.half(), q, dual(s), z),
+                     lambda: ops.native_grouped_matmul(dual(x), w, ends),
+                     lambda: torch.autograd.grad(y, leaf, dual(torch.ones_like(y)), retain_graph=True)):
+            with pytest.raises(RuntimeError, match="forward.mode|jvp"):
+                call()
+        assert ops.grouped_matmul(x, w, ends).shape == (4, 8)
