@@ -67,6 +67,12 @@ def _needs_build(out: Path, deps) -> bool:
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+def kernel_flags():
+    """What every kernel source is compiled with (the static checks of the generated code too)."""
+    return [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
+            "-Wno-unused-result", "-munsafe-fp-atomics", f"-I{CSRC}", *NO_PACKED_F32]
+
+
 def experiments() -> bool:
     """``PDMB_EXPERIMENTS=1``: also compile the A/B and timing-only diagnostic
     kernels (api.h ``ExperimentKernel``). The default build ships without them."""
@@ -192,8 +198,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
     import torch
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    hip_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
-                 "-Wno-unused-result", "-munsafe-fp-atomics", f"-I{CSRC}", *NO_PACKED_F32]
+    hip_flags = kernel_flags()
     if experiments():
         hip_flags.append("-DPDMB_EXPERIMENTS=1")
     host_flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",

@@ -1,10 +1,13 @@
 """One gfx950 compile per (source, build flavour) per test process, shared by
-the static assembly checks (test_kernel_asm.py, test_mfma_hazards.py)."""
+the static assembly checks (test_kernel_asm.py, test_mfma_hazards.py), with the
+flags that the library itself is compiled with."""
 import functools
 import os
 import shutil
 import subprocess
 import tempfile
+
+from pytorch_distributed_matmul_benchmark_amd.ops.build import kernel_flags
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                     "pytorch_distributed_matmul_benchmark_amd", "ops", "csrc")
@@ -18,7 +21,7 @@ def gfx950_asm(src: str, experiments: bool = False) -> str:
     d = tempfile.mkdtemp(prefix="pdmb_asm_")
     try:
         defs = ["-DPDMB_EXPERIMENTS=1"] if experiments else []
-        subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", f"-I{CSRC}", *defs, "-c",
+        subprocess.run([HIPCC, *kernel_flags(), *defs, "-c",
                         os.path.join(CSRC, src), "-o", os.path.join(d, "k.o"), "-save-temps"],
                        cwd=d, check=True, capture_output=True, timeout=900)
         s = next(f for f in os.listdir(d) if "gfx950" in f and f.endswith(".s"))
