@@ -21,7 +21,8 @@ def gfx950_asm(src: str, experiments: bool = False) -> str:
     d = tempfile.mkdtemp(prefix="pdmb_asm_")
     try:
         defs = ["-DPDMB_EXPERIMENTS=1"] if experiments else []
-        subprocess.run([HIPCC, *kernel_flags(), *defs, "-c",
+        lang = ["-x", "hip"] if src.endswith(".cpp") else []
+        subprocess.run([HIPCC, *kernel_flags(), *defs, *lang, "-c",
                         os.path.join(CSRC, src), "-o", os.path.join(d, "k.o"), "-save-temps"],
                        cwd=d, check=True, capture_output=True, timeout=900)
         s = next(f for f in os.listdir(d) if "gfx950" in f and f.endswith(".s"))
