@@ -66,3 +66,42 @@ def test_refusals_name_their_reason():
         ops.int4_matmul(x, q, s, out=torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(2, 1))
     with pytest.raises(RuntimeError, match="gradient"):
         ops.int4_matmul(x, q, s, out=torch.zeros(2, 1, device="cuda", dtype=torch.bfloat16, requires_grad=True))
+
+
+def _whole(lead, M, N, K, G, dtype, zero):
+    """x of -3 .. 3, scales 1/4 .. 2: a group's sum stays below 128 x 3 x 31 and the sum of all, in quarters, below
+    4 x 2 x 3 x 15 K < 2^24 for K up to 46603."""
+    assert 4 * 2 * 3 * 15 * K < 2 ** 24
+    q, s, z = _weight(lead, N, K, G, dtype, zero)
+    s = 2.0 ** torch.randint(-2, 2, s.shape, device="cuda").to(dtype)
+    return torch.randint(-3, 4, (M, K), device="cuda").to(dtype), q, s, z
+
+
+# long sums, partial last chunks (K % 128 = 32, 64, 96) and every group size, on each kernel and tile height
+@pytest.mark.parametrize("M,N,K,G", [
+    (1, 4096, 4096, 128), (1, 4096, 4096, 32), (1, 8200, 8192, 128), (4, 8300, 6208, 64), (13, 8300, 6272, 128),
+    (13, 8300, 6240, 32), (16, 11007, 4096, 32), (16, 1023, 1024, 256), (17, 130, 544, 32), (32, 256, 2048, 2048),
+    (25, 1024, 5600, 32), (33, 5400, 2080, 32), (47, 10176, 4480, 128), (64, 8001, 672, 32), (100, 8192, 4096, 64),
+    (100, 384, 1536, 512), (130, 5000, 1152, 64), (500, 4090, 768, 128), (515, 640, 1056, 32)])
+@pytest.mark.parametrize("zero", [False, True], ids=["sym", "zero"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_whole_numbers(dtype, zero, M, N, K, G):
+    x, q, s, z = _whole((), M, N, K, G, DT[dtype], zero)
+    y = ops.int4_matmul(x, q, s, z)
+    _same(y, x, q, s, z)
+    # (one matrix instruction's k less would show)
+    assert not torch.equal(y, (x[:, :-32].double() @ _values(q, s, z)[0].t()[:-32]).to(y.dtype))
+
+
+@pytest.mark.parametrize("sizes,N,K,G", [
+    ([1] * 66, 1408, 2048, 128), ([0, 3, 1, 0], 8192, 6240, 32), ([17, 0, 40, 2], 100, 416, 32),
+    ([100, 64, 1, 70], 4100, 4192, 32), ([30, 0, 32, 20], 5000, 1024, 64), ([9] * 8, 1416, 4128, 32)])
+@pytest.mark.parametrize("zero", [False, True], ids=["sym", "zero"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_whole_numbers_of_experts(dtype, zero, sizes, N, K, G):
+    x, q, s, z = _whole((len(sizes),), sum(sizes), N, K, G, DT[dtype], zero)
+    y = ops.int4_matmul(x, q, s, z, ends=torch.tensor(sizes).cumsum(0).cuda())
+    lo = 0
+    for e, n in enumerate(sizes):
+        _same(y[lo:lo + n], x[lo:lo + n], q[e], s[e], None if z is None else z[e])
+        lo += n
