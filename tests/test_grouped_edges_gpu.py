@@ -97,3 +97,50 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(RuntimeError, match="forward.mode|jvp"):
                 call()
         assert ops.grouped_matmul(x, w, ends).shape == (4, 8)
+
+
+def _far(t, at=3):
+    """t with its last dimension's rows more than 8 MB apart, at an odd element, NaN between them."""
+    b = torch.full((*t.shape[:-1], (1 << 23) // t.element_size() + 9), float("nan"), device="cuda", dtype=t.dtype)
+    b[..., at:at + t.shape[-1]] = t
+    return b[..., at:at + t.shape[-1]]
+
+
+# from few rows to many, short sums and long ones (which several sets of waves share)
+@pytest.mark.parametrize("sizes,K,N", [
+    ([2, 0, 3], 70, 40), ([1], 1, 3), ([2, 0, 3], 1101, 37), ([20, 0, 13], 2056, 40), ([40, 0, 50], 1101, 37),
+    ([100, 50, 70], 1101, 136), ([100, 50, 70], 201, 37), ([600, 700], 130, 40)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_rows_far_apart(dtype, sizes, K, N):
+    """Strides past 8 MB, which are read by the element at the edges: of the rows, of the weights in both
+    layouts, of what the weights' gradient sums."""
+    T, E, ends = sum(sizes) + 2, len(sizes), _ends(sizes)
+    x, w = _data(T, K, N, E, DT[dtype])
+    dy, _ = _data(T, N, 1, 1, DT[dtype], seed=3)
+    x[T - 2:], dy[T - 2:] = float("nan"), float("inf")
+    x0, dy0 = x.nan_to_num(), dy.nan_to_num(posinf=0)
+    want = _rows_exact(x0, w, ends), _rows_exact(x0.abs(), w.abs(), ends), K
+    if T <= 300:
+        _close(ops.grouped_matmul(_far(x), w, ends), *want)
+        _close(ops.grouped_weight_grad(_far(x), _far(dy), ends), _reduce_exact(x0, dy0, ends),
+               _reduce_exact(x0.abs(), dy0.abs(), ends), max(sizes))
+    if K <= 300:
+        _close(ops.grouped_matmul(x, _far(w), ends), *want)
+    _close(ops.grouped_matmul(x, _far(w.transpose(1, 2)).transpose(1, 2), ends), *want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_many_rows_and_long_gradients_far_apart(dtype):
+    x, w = _data(6000, 72, 1200, 1, DT[dtype])
+    ends = _ends([5990])
+    y = ops.grouped_matmul(x, _far(w.transpose(1, 2)).transpose(1, 2), ends)
+    _close(y, _rows_exact(x, w, ends), _rows_exact(x.abs(), w.abs(), ends), 72)
+    x, _ = _data(1700, 40, 1, 1, DT[dtype])
+    dy, _ = _data(1700, 70, 1, 1, DT[dtype], seed=3)
+    ends = _ends([1000, 650])
+    _close(ops.grouped_weight_grad(_far(x), dy, ends), _reduce_exact(x, dy, ends),
+           _reduce_exact(x.abs(), dy.abs(), ends), 1000)
+    both, out = w[:, :70, :40].expand(2, -1, -1), torch.full((1700, (1 << 23) // x.element_size() + 9), 2.0,
+                                                            device="cuda", dtype=DT[dtype])[:, 1:41]
+    ops.grouped_matmul(dy, both, ends, out=out)
+    assert torch.equal(out[:1650], ops.grouped_matmul(dy, both, ends)[:1650]) and bool((out[1650:] == 2).all())
