@@ -71,7 +71,8 @@ def native_grouped_matmul(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) 
     w[e]^T`` on the same kernel (the transposed weights are read in place) and
     ``dw[e] = x_e^T @ dy_e`` (``grouped.grouped_weight_grad``). Rows behind the last
     expert's, and experts without rows, get zero gradients. ``ends`` must not
-    change between the forward and the backward pass. Under a stream capture a leaf
-    whose graph from the default stream is still alive is refused."""
+    change between the forward and the backward pass. Under a stream capture an
+    operand is refused that is, or was computed from, a leaf whose graph from the default
+    stream is still alive."""
     res = grouped._native_call("grouped_node", x, w, ends)
     return _NativeGroupedMatmul.apply(x, w, ends) if res is None else res

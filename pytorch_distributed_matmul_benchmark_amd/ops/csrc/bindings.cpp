@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <cstdlib>
+#include <unordered_set>
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -481,23 +482,36 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
 
 // While an eager graph of a leaf lives, the leaf's gradient belongs to the stream of that
 // graph. The default stream cannot join a capture, and the backward pass finds that out
-// in a thread of its own, which ends the process: refused here, before it comes to that.
-void refuse_eager_leaf(const at::Tensor& t) {
-  if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf() || !at::GradMode::is_enabled()) return;
+// in a thread of its own, which ends the process: refused here, before it comes to that,
+// for the operand itself and for all that it was computed from (a view or a cast of a weight).
+void refuse_eager_graph(const at::Tensor& t) {
+  if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !at::GradMode::is_enabled()) return;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   check_hip(hipStreamIsCapturing(c10::hip::getCurrentHIPStream(t.device().index()).stream(), &status),
             "hipStreamIsCapturing");
   if (status == hipStreamCaptureStatusNone) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  const auto stream = node ? node->stream() : c10::nullopt;
-  TORCH_CHECK(!stream || stream->id() != 0,
-              "native_grouped_matmul: a graph of the same leaf tensor, made on the default stream, is still alive: "
-              "release it (its result and what was computed from it) before this capture");
+  const auto first = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  auto visit = [&](torch::autograd::Node* n) {
+    if (n && seen.insert(n).second) todo.push_back(n);
+  };
+  visit(first.get());
+  while (!todo.empty()) {
+    torch::autograd::Node* n = todo.back();
+    todo.pop_back();
+    const auto stream = n->stream();
+    TORCH_CHECK(!stream || stream->id() != 0,
+                "native_grouped_matmul: a graph made on the default stream, of a leaf tensor that an operand is or comes "
+                "from, is still alive: release it (its results and what was computed from them) before this capture, and "
+                "compute the operand inside it");
+    for (const auto& e : n->next_edges()) visit(e.function.get());
+  }
 }
 
 MaybeTensor grouped_node(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ends) {
-  refuse_eager_leaf(x);
-  refuse_eager_leaf(w);
+  refuse_eager_graph(x);
+  refuse_eager_graph(w);
   pdmb::GroupedProblem p{};
   if (!rows_problem(x, w, ends, p)) return {};
   return GroupedNode::apply(x, w, ends, p);

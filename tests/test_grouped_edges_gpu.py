@@ -144,3 +144,44 @@ def test_many_rows_and_long_gradients_far_apart(dtype):
                                                             device="cuda", dtype=DT[dtype])[:, 1:41]
     ops.grouped_matmul(dy, both, ends, out=out)
     assert torch.equal(out[:1650], ops.grouped_matmul(dy, both, ends)[:1650]) and bool((out[1650:] == 2).all())
+
+
+@pytest.mark.parametrize("derive", [lambda w: w.transpose(1, 2), lambda w: w.bfloat16().transpose(1, 2),
+                                    lambda w: (w * 2).transpose(1, 2)], ids=["view", "cast", "computed"])
+def test_capture_beside_a_living_eager_graph_of_what_an_operand_comes_from(derive):
+    """A weight that is used through a view or a cast: the leaf behind it decides."""
+    leaf = torch.randn(2, 24, 16, device="cuda", requires_grad=True)
+    ends = torch.tensor([2, 4], device="cuda")
+    x = torch.randn(4, 16, device="cuda").to(derive(leaf.detach()).dtype)
+    alive = ops.native_grouped_matmul(x, derive(leaf), ends)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.native_grouped_matmul(x, derive(leaf), ends)
+    eager = derive(leaf)
+    del alive
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):  # the operand's own graph, from before the capture
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.native_grouped_matmul(x, eager, ends)
+    del eager
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = ops.native_grouped_matmul(x, derive(leaf), ends)
+        torch.autograd.grad(y, leaf, torch.ones_like(y))
+        del y
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.native_grouped_matmul(x, derive(leaf), ends)
+        (dw,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    for i in range(3):
+        with torch.no_grad():
+            leaf.add_(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        again = leaf.detach().clone().requires_grad_()
+        want = ops.native_grouped_matmul(x, derive(again), ends)
+        assert torch.equal(y, want)
+        assert torch.equal(dw, torch.autograd.grad(want, again, torch.ones_like(want))[0])
