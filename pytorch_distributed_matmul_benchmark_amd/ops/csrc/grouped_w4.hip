@@ -72,7 +72,9 @@ __device__ __forceinline__ void mfma_first(f32x4& acc, const s16x8& b, const s16
 }
 
 // One LDS-DMA piece (64 lanes x 16 B) to lds0w + OFF, lane offsets only. The
-// s_nop keeps 5 wait states between an SGPR restored by v_readlane and the load.
+// s_nop keeps 5 wait states between an SGPR restored by v_readlane and the load: the next tile's
+// operands and the search do not fit beside the loop's descriptors where an operand is KS, and 20 (row-major B)
+// or 47 (reduce) SGPRs wait in lanes of a vector register. No vector register spills.
 __device__ __forceinline__ void dma_piece(u32x4 rsrc, uint32_t voff, uint32_t lds0w, int off) {
   asm volatile(
       "s_add_u32 m0, %2, %3\n\t"
