@@ -15,7 +15,7 @@
 // scaled once, in fp32.
 //
 // So a bf16 sum's terms are x (16 + q) and -x (16 + zero), not x (q - zero): its fp32 error is relative to
-// |x| (32 + q + zero) (B = 128 for nibble 0, which needs no shift, is one instruction in 36 less and
+// |x| (32 + q + zero) (B = 128 for nibble 0, which needs no shift, is one instruction a dword less and
 // made that up to eight times as much), a row whose 31 sum |x| over a group passes 3.4e38 gives NaN, and so
 // does a row with an infinity: the two products cancel.
 //
@@ -32,10 +32,10 @@
 //
 // Two kernels: gemm_int4_few for 16 rows a tile and short sums or narrow weights, and
 // gemm_int4_rows for more, where the rows of a block come through LDS once for 64 columns.
-// What bounds them: 1 row, 8192 x 16384: 14.7 us, the read of the weight (4.7 TB/s) with 7 us of
+// What bounds them: 1 row, 8192 x 16384: 14.9 us, the read of the weight (4.6 TB/s) with 7 us of
 // widening beside it; 16 rows, 4096 x 11007, groups of 32: 11.4 us, of which the vector
-// units work 5.3 (36 instructions for an MFMA) and the rest is launch, first loads and the
-// join; 100 rows, 4096 x 8192: 21.5 us, vector units 9.5, matrix units 7 (two products for
+// units work 5.0 (34 instructions for an MFMA) and the rest is launch, first loads and the
+// join; 100 rows, 4096 x 8192: 21.8 us, vector units 9.7, matrix units 7 (two products for
 // a bf16 weight) and LDS 5, which overlap little with a barrier a step.
 #include "api.h"
 #include "grouped.h"
@@ -380,7 +380,8 @@ __device__ __forceinline__ void few_sums(const Args& a, const RowTile& r, int n0
 }
 
 // (Scheduled for four waves a SIMD, which is what a grid has of it: 64 experts 2048 x 2048 of 64 rows
-// 27.3 -> 25.2 us, 16 x 4096 x 11007 12.8 -> 12.3.)
+// 27.3 -> 25.2 us, 16 x 4096 x 11007 12.8 -> 12.3. 32 columns with groups of 32 or 64 need the registers of two, or
+// they go to scratch.)
 template <int DT, int NB, int SG, int RX, bool ZERO, int W, int D>
 __attribute__((amdgpu_waves_per_eu(NB > 1 && SG > 1 ? 2 : 4, 4)))
 __global__ void __launch_bounds__(64 * W) gemm_int4_few(Args a) {
@@ -643,7 +644,7 @@ hipError_t pick_few(const Args& a, hipStream_t s) {
   // waves a ns (16 x 4096 x 11007: 4 waves 11.7 us, 2 15.0; 64 experts 2048 x 2048 of
   // 64 rows, 32 columns a tile: 2 waves 27 us, 4 29, 8 43; 16 columns and 2 waves 30).
   const long long tiles = tiles_about(a, 16) * ((a.N + 15) / 16);
-  // Long sums of many tiles: 8 waves on 32 columns (1 x 8192 x 16384: 14.7 us, 4 on 16 15.6;
+  // Long sums of many tiles: 8 waves on 32 columns (1 x 8192 x 16384: 14.9 us, 4 on 16 15.6;
   // 8 rows 18.5, 20; 64 rows of 16 experts 8192 x 2048 37, 42; but 77 of 8, 4128 x 1416: 14.8, 13.1).
   if (tiles >= 4096) return launch_few<DT, 2, SG, RX, ZERO, 2>(a, s);
   if (tiles > 512 && a.K >= 48 * 128) return launch_few<DT, 2, SG, RX, ZERO, 8>(a, s);

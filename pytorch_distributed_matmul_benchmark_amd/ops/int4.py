@@ -10,7 +10,7 @@ multiple of 128, and divides K. Expert weights have a leading dimension [E, ...]
 
 GPU tensors run on ``csrc/int4.hip``: the values are multiplied as whole numbers,
 each group's fp32 sum is scaled in fp32, and the result is rounded once. They are
-made for the rows of a serving batch (100 rows, 4096 x 8192: 22 us); from some hundreds of
+made for the rows of a serving batch (100 rows, 4096 x 8192: 22 us); from about a hundred
 rows ``matmul`` with a weight kept as ``int4_dequantize`` returns it is faster. CPU
 tensors use ``torch.matmul`` on the dequantised weight.
 """
