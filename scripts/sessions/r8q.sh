@@ -1,5 +1,5 @@
 #!/bin/bash
-# Round 6 session Q (PDMB_EXPERIMENTS=1 build in the tree): the lean exact-fp32
+# Session Q (PDMB_EXPERIMENTS=1 build in the tree): the lean exact-fp32
 # W4 K-loop (x_f32_w4_lean2), the settled A/B against the auto kernel
 # (f32_t128x2) and hipBLASLt on the full grids, two sessions; then PMC at 16k.
 # (The streamed kernel this session also ran is not launched any more.)

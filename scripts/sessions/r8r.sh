@@ -1,5 +1,5 @@
 #!/bin/bash
-# Round 6 session R (PDMB_EXPERIMENTS=1 build in the tree): the lean exact-fp32
+# Session R (PDMB_EXPERIMENTS=1 build in the tree): the lean exact-fp32
 # W4 K-loop (x_f32_w4_lean2; the streamed kernel this session also ran is not launched any more)
 # against the auto kernel and hipBLASLt on the whole-tile fp32 grids beyond the
 # three squares: the matrix_parallel shards of 8k / 16k at ws = 2 / 4 / 8, more
