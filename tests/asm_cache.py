@@ -5,7 +5,6 @@ import functools
 import os
 import shutil
 import subprocess
-import tempfile
 
 from pytorch_distributed_matmul_benchmark_amd.ops.build import kernel_flags
 
@@ -14,19 +13,16 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 HIPCC = "/opt/rocm/bin/hipcc" if os.path.exists("/opt/rocm/bin/hipcc") else shutil.which("hipcc")
 
 
-@functools.lru_cache(maxsize=None)
 def gfx950_asm(src: str, experiments: bool = False) -> str:
     """The device assembly (.s text) of ``csrc/src`` (default build, or with the
     A/B experiment kernels)."""
-    d = tempfile.mkdtemp(prefix="pdmb_asm_")
-    try:
-        defs = ["-DPDMB_EXPERIMENTS=1"] if experiments else []
-        lang = ["-x", "hip"] if src.endswith(".cpp") else []
-        subprocess.run([HIPCC, *kernel_flags(), *defs, *lang, "-c",
-                        os.path.join(CSRC, src), "-o", os.path.join(d, "k.o"), "-save-temps"],
-                       cwd=d, check=True, capture_output=True, timeout=900)
-        s = next(f for f in os.listdir(d) if "gfx950" in f and f.endswith(".s"))
-        with open(os.path.join(d, s)) as fh:
-            return fh.read()
-    finally:
-        shutil.rmtree(d, ignore_errors=True)
+    return _compile(src, experiments)
+
+
+@functools.lru_cache(maxsize=None)
+def _compile(src: str, experiments: bool) -> str:
+    defs = ["-DPDMB_EXPERIMENTS=1"] if experiments else []
+    lang = ["-x", "hip"] if src.endswith(".cpp") else []
+    r = subprocess.run([HIPCC, *kernel_flags(), *defs, *lang, "-S", "--cuda-device-only", os.path.join(CSRC, src), "-o", "-"],
+                       check=True, capture_output=True, text=True, timeout=900)
+    return r.stdout

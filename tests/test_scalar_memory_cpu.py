@@ -4,6 +4,7 @@ import re
 
 import pytest
 from asm_cache import HIPCC, gfx950_asm
+from test_grouped_asm import SOURCES, _asm
 
 from pytorch_distributed_matmul_benchmark_amd.ops import build
 
@@ -23,6 +24,6 @@ def test_the_check_sees_a_write():
 @pytest.mark.skipif(HIPCC is None, reason="hipcc not available")
 @pytest.mark.parametrize("src", build.HIP_SOURCES)
 def test_scalar_memory_is_only_read(src):
-    asm = gfx950_asm(src)
+    asm = _asm(src) if src in SOURCES else gfx950_asm(src)
     assert "s_load_" in asm
     assert not others(asm)
